@@ -214,6 +214,100 @@ int lrs_timer_start(lrs_ctx *ctx);
 int lrs_timer_stop(lrs_ctx *ctx, float *ms);
 
 /* ------------------------------------------------------------------------ */
+/* sampled and speculated decoding                                          */
+/* ------------------------------------------------------------------------ */
+/* One token of each row of logits [rows][ld] (vocab of each) from a given
+ * random number u_dev[row] in [0, 1): Sampler::sample
+ * (llama-sampling/src/sampler.rs:24-88) on the device, with min-p.  With a
+ * row's words in the order logit descending, index ascending, and weights
+ * w = e^((l - l_max) / temperature):
+ *   top_k  keeps the first top_k words (0: all),
+ *   top_p  of those the shortest prefix whose weights sum to at least top_p
+ *          times theirs (1: all; at least one word),
+ *   min_p  of those the words with w >= min_p (0: all);
+ * the token is the least index i whose kept words j <= i sum to more than u
+ * times all kept words' sum.  temperature 0 takes the first word (argmax).
+ * -inf (a masked word) and NaN are never taken; a row with nothing else gives
+ * LRS_NO_TOKEN and probability 0.  u below 0 or NaN counts as 0, u >= 1 takes
+ * the last kept word.  probs_dev (may be NULL): the token's share of the kept
+ * words' sum.  Weights are summed as whole multiples of 2^-42 of the largest, so
+ * that a call's results are always the same; words of less than half of that
+ * are not drawn.  Async on the context stream; uses the context scratch (at
+ * most 65 KB a row). */
+#define LRS_NO_TOKEN 0xFFFFFFFFu
+#define LRS_SAMPLE_MAX_VOCAB 2097152u
+typedef struct {
+    float temperature;
+    uint32_t top_k;
+    float top_p, min_p;
+} lrs_sampling;
+int lrs_sample_dev(lrs_ctx *ctx, const float *logits_dev, size_t ld, uint32_t rows, uint32_t vocab,
+                   const lrs_sampling *p, const float *u_dev, uint32_t *tokens_dev, float *probs_dev);
+
+/* An f16 cache on the device: k and v [n_kv][rows][head_dim], 16-byte aligned,
+ * head_dim 64, 128 or 256 (the layout of the models' own). */
+typedef struct {
+    void *k, *v;
+    uint32_t n_kv, rows, head_dim;
+} lrs_kv;
+
+/* Rotation: pair i of the first rope_dim dims of a head, dims (2i, 2i + 1)
+ * (LRS_ROPE_PAIRS, rope_norm, ops.rs:952-975) or (i, i + rope_dim / 2)
+ * (LRS_ROPE_HALVES), turns by position * freq[i] and is multiplied by scale.
+ * The angle is reduced in double; with f32_angle it is rounded to f32 first, as
+ * the models' own decode and prompt calls do. */
+#define LRS_ROPE_PAIRS 0u
+#define LRS_ROPE_HALVES 1u
+typedef struct {
+    uint32_t rope_dim, layout;
+    int f32_angle;
+    float scale;
+} lrs_rope;
+/* Frequencies on the host: freq[rope_dim / 2] and the scale that goes with them.
+ * LRS_ROPE_PLAIN: base^(-2i / rope_dim); LRS_ROPE_LINEAR: those / factor;
+ * LRS_ROPE_YARN: pairs that make more than beta_fast turns over orig_ctx
+ * positions as plain, below beta_slow as linear, between them by a ramp over
+ * the pairs, and scale 1 + 0.1 ln(factor). */
+#define LRS_ROPE_PLAIN 0u
+#define LRS_ROPE_LINEAR 1u
+#define LRS_ROPE_YARN 2u
+typedef struct {
+    uint32_t type;
+    float base, factor;
+    uint32_t orig_ctx;
+    float beta_fast, beta_slow;
+} lrs_rope_scaling;
+int lrs_rope_freqs(uint32_t rope_dim, const lrs_rope_scaling *sc, float *freq, float *scale);
+/* n tokens (at most 65535) at positions pos_dev[n]: q rotated into q_out
+ * [n][n_head * head_dim] (may be q_dev where ldq is its row), k rotated and v
+ * rounded to f16 into row slot_dev[t] of every KV head.  q, k and v are rows of
+ * ldq, ldk, ldv floats.  A slot past the cache's rows (a padded token) stores
+ * nothing; the slots of a call differ.  Rows that no slot names are left as they
+ * were.  Async on the context stream, no scratch. */
+int lrs_rope_append_dev(lrs_ctx *ctx, const lrs_kv *kv, const lrs_rope *rope, const float *freq_dev, const float *q_dev,
+                        size_t ldq, const float *k_dev, size_t ldk, const float *v_dev, size_t ldv,
+                        const uint32_t *pos_dev, const uint32_t *slot_dev, uint32_t n, uint32_t n_head, float *q_out_dev);
+
+/* A tree of n drafted tokens: parents[i] < i, or LRS_NO_PARENT for a child of
+ * the last cached position.  lrs_tree_mask (host): mask [n][ceil(n / 32)] with
+ * bit j of row i set where node j is i or an ancestor of it, depth[n] (may be
+ * NULL) from 0. */
+#define LRS_TREE_MAX 512u
+#define LRS_NO_PARENT 0xFFFFFFFFu
+int lrs_tree_mask(const uint32_t *parents, uint32_t n, uint32_t *mask, uint32_t *depth);
+/* Grouped-query attention of n tokens (at most LRS_TREE_MAX) whose K and V are in
+ * the cache's rows len..len + n - 1: token i sees rows 0..len - 1 and the rows
+ * len + j whose bit j of mask_dev row i is set (NULL: j <= i).  out[i][h] =
+ * sum p V / sum p, p = e^(scale q K), in the f32 grade of the prompt path (f16
+ * cache exact, q and p to 22 bits, f32 sums); a token that sees nothing has
+ * zeros.  What a token does not see does not reach it, NaN and inf included.
+ * q_dev, out_dev [n][n_head * head_dim], 16-byte aligned, not the same.  Async
+ * on the context stream; uses at most 8 MB of the context scratch, its first
+ * size. */
+int lrs_attn_tree_dev(lrs_ctx *ctx, const lrs_kv *kv, const float *q_dev, uint32_t n, uint32_t n_head, uint32_t len,
+                      const uint32_t *mask_dev, float scale, float *out_dev);
+
+/* ------------------------------------------------------------------------ */
 /* model level: llama_model::GpuResidentDecode                              */
 /* (crates/llama-model/src/gpu.rs:379-455) as implemented by                 */
 /* llama_vulkan::ResidentForward (resident_forward.rs:5223-5282)             */
@@ -328,6 +422,35 @@ int lrs_decode_greedy(lrs_model *m, uint32_t token, uint32_t pos, uint32_t *next
  * on the device with no host round trip per token (out_tokens[n_gen]). */
 int lrs_generate_greedy(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uint32_t pos0,
                         uint32_t n_gen, uint32_t *out_tokens);
+/* decode + sampling on the device (lrs_sample_dev's rule, u in [0, 1)).  A row
+ * of logits without a word that can be taken fails with LRS_E_HIP. */
+int lrs_decode_sample(lrs_model *m, uint32_t token, uint32_t pos, const lrs_sampling *p, float u, uint32_t *next);
+/* lrs_generate_greedy with every token sampled: token i of out_tokens[n_gen]
+ * from u[i], with no host round trip per token. */
+int lrs_generate_sample(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uint32_t pos0, uint32_t n_gen,
+                        const lrs_sampling *p, const float *u, uint32_t *out_tokens);
+/* A tree of n drafted tokens in one pass over the weights (dense models whose
+ * batch_size() is above 1): node i (parents as in lrs_tree_mask) at position
+ * pos0 + its depth, in cache slot pos0 + i, attends positions 0..pos0 - 1 and its
+ * ancestors.  logits (may be NULL): [n][vocab], every node's.  The cache length
+ * becomes pos0: lrs_tree_keep then takes a path of the tree into it, any other
+ * call drops the tree. */
+int lrs_decode_tree(lrs_model *m, const uint32_t *tokens, const uint32_t *parents, uint32_t n, uint32_t pos0,
+                    float *logits);
+/* Keeps nodes[0..n_nodes) of the last tree, each the parent of the next, the
+ * first without one: their K / V rows move to pos0.. and the cache length
+ * becomes pos0 + n_nodes. */
+int lrs_tree_keep(lrs_model *m, const uint32_t *nodes, uint32_t n_nodes);
+/* Speculative decoding's step, on the device: the tree (node 0 its only root:
+ * the last token, not yet cached) as lrs_decode_tree; a token sampled at every
+ * node i from u[i] (NULL: temperature must be 0); from node 0 on, a node's
+ * sampled token is the next one and its first child that drafted it the next
+ * node.  out_tokens[n]: the n_out tokens of that walk (1 at least), of which all
+ * but the last are cached with node 0's; the last is the next root.  Rejected
+ * rows are dropped.  A sampled token that no child drafted still counts, so the
+ * tokens are distributed as those of lrs_decode_sample. */
+int lrs_verify_tree(lrs_model *m, const uint32_t *tokens, const uint32_t *parents, uint32_t n, uint32_t pos0,
+                    const lrs_sampling *p, const float *u, uint32_t *out_tokens, uint32_t *n_out);
 /* Per-op timing of the decode plan (the LLAMA_RS_PROFILE timestamps of
  * resident_forward.rs:3141-3149, 4556-4745): launches `op` for layers
  * 0,1,2,.. in turn `iters` times on the model stream, outside the graph, and

@@ -35,6 +35,33 @@ TYPE_NAME = {F32: "F32", F16: "F16", Q4_0: "Q4_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q
 NOALLOC_MAX_N_IN = 46592
 
 
+# sampled and speculated decoding (lrs.h)
+NO_TOKEN = NO_PARENT = 0xFFFFFFFF
+TREE_MAX = 512
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "yarn": 2}
+
+
+class LrsSampling(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_uint32), ("top_p", C.c_float),
+                ("min_p", C.c_float)]
+
+
+class LrsKv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_kv", C.c_uint32), ("rows", C.c_uint32),
+                ("head_dim", C.c_uint32)]
+
+
+class LrsRope(C.Structure):
+    _fields_ = [("rope_dim", C.c_uint32), ("layout", C.c_uint32), ("f32_angle", C.c_int),
+                ("scale", C.c_float)]
+
+
+class LrsRopeScaling(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("base", C.c_float), ("factor", C.c_float),
+                ("orig_ctx", C.c_uint32), ("beta_fast", C.c_float), ("beta_slow", C.c_float)]
+
+
 class ModelError(RuntimeError):
     """Mirror of llama_model::ModelError::Gpu(String)."""
 
@@ -72,6 +99,12 @@ def _load() -> C.CDLL:
         "lrs_gemm_group_dev": (i32, [vp, vp, u32, vp, vp, u32, i32]),
         "lrs_quantize_q8_0_dev": (i32, [vp, vp, u32, i32, vp]),
         "lrs_matvec_q8_0_actq_dev": (i32, [vp, vp, vp, vp, u32, i32]),
+        "lrs_sample_dev": (i32, [vp, vp, sz, u32, u32, C.POINTER(LrsSampling), vp, vp, vp]),
+        "lrs_rope_freqs": (i32, [u32, C.POINTER(LrsRopeScaling), vp, C.POINTER(C.c_float)]),
+        "lrs_rope_append_dev": (i32, [vp, C.POINTER(LrsKv), C.POINTER(LrsRope), vp, vp, sz, vp, sz,
+                                      vp, sz, vp, vp, u32, u32, vp]),
+        "lrs_tree_mask": (i32, [vp, u32, vp, vp]),
+        "lrs_attn_tree_dev": (i32, [vp, C.POINTER(LrsKv), vp, u32, u32, u32, vp, C.c_float, vp]),
         "lrs_dev_alloc": (i32, [vp, sz, pvp]),
         "lrs_dev_free": (i32, [vp, vp]),
         "lrs_copy_h2d": (i32, [vp, vp, vp, sz]),
@@ -384,6 +417,97 @@ def gemm_group(ctx: Context, weights, a: np.ndarray, precision: int = 1) -> list
         ab.free()
         for y in ys:
             y.free()
+
+
+def sampling(temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+             min_p: float = 0.0) -> LrsSampling:
+    if not 0 <= top_k <= 0xFFFFFFFF:
+        raise ModelError(-1, "top_k must be 0 (all) or a count")
+    return LrsSampling(temperature, top_k, top_p, min_p)
+
+
+def sample_dev(ctx: Context, logits, rows: int, vocab: int, u, tokens, probs=None, ld: int | None = None,
+               **options) -> None:
+    """lrs_sample_dev (async, device buffers): one token of each row of logits
+    [rows][ld] from u [rows] f32; tokens [rows] u32, probs [rows] f32 or None.
+    options: temperature, top_k, top_p, min_p (:func:`sampling`)."""
+    check(lib.lrs_sample_dev(ctx.h, logits.ptr, vocab if ld is None else ld, rows, vocab,
+                             C.byref(sampling(**options)), u.ptr, tokens.ptr, probs.ptr if probs else None))
+
+
+def sample(ctx: Context, logits: np.ndarray, u, **options):
+    """Host wrapper of sample_dev: logits [rows, vocab], u [rows] ->
+    (tokens [rows] u32, probabilities [rows] f32)."""
+    x = np.ascontiguousarray(logits, dtype=np.float32)
+    u = np.ascontiguousarray(u, dtype=np.float32)
+    if x.ndim != 2 or u.shape != x.shape[:1]:
+        raise ModelError(-1, "logits are [rows, vocab], u is [rows]")
+    rows, vocab = x.shape
+    bufs = [ctx.alloc(x.nbytes), ctx.alloc(u.nbytes), ctx.alloc(4 * rows), ctx.alloc(4 * rows)]
+    try:
+        bufs[0].upload(x)
+        bufs[1].upload(u)
+        sample_dev(ctx, bufs[0], rows, vocab, bufs[1], bufs[2], bufs[3], **options)
+        ctx.sync()
+        return bufs[2].download(np.uint32, rows), bufs[3].download(np.float32, rows)
+    finally:
+        for b in bufs:
+            b.free()
+
+
+def rope_freqs(rope_dim: int, base: float, scaling: str = "plain", factor: float = 1.0, orig_ctx: int = 0,
+               beta_fast: float = 32.0, beta_slow: float = 1.0):
+    """lrs_rope_freqs: (freq [rope_dim / 2] f32, scale) of a rotation, plain or
+    scaled for contexts of factor times orig_ctx ("linear", "yarn")."""
+    if scaling not in ROPE_SCALINGS:
+        raise ModelError(-1, f"unknown rope scaling {scaling!r}")
+    freq, scale = np.empty(max(rope_dim // 2, 1), np.float32), C.c_float()
+    check(lib.lrs_rope_freqs(rope_dim, C.byref(LrsRopeScaling(ROPE_SCALINGS[scaling], base, factor, orig_ctx,
+                                                              beta_fast, beta_slow)), _ptr(freq), C.byref(scale)))
+    return freq, scale.value
+
+
+class KvCache:
+    """An f16 cache on the device: k and v buffers of [n_kv][rows][head_dim]
+    (lrs_kv); the buffers stay the caller's."""
+
+    def __init__(self, k, v, n_kv: int, rows: int, head_dim: int):
+        need = 2 * n_kv * rows * head_dim
+        if k.nbytes < need or v.nbytes < need:
+            raise ModelError(-1, f"a cache of {n_kv} x {rows} x {head_dim} needs {need} bytes per buffer")
+        self.buffers = (k, v)
+        self.c = LrsKv(k.ptr, v.ptr, n_kv, rows, head_dim)
+
+
+def rope_append_dev(ctx: Context, kv: KvCache, freq, rope_dim: int, q, k, v, pos, slot, n: int, n_head: int, q_out,
+                    layout: int = ROPE_PAIRS, scale: float = 1.0, f32_angle: bool = False, ldq: int | None = None,
+                    ldk: int | None = None, ldv: int | None = None) -> None:
+    """lrs_rope_append_dev (async, device buffers): n tokens' q and k rotated at
+    positions pos [n], q into q_out, k and v as f16 into the cache's rows slot [n]."""
+    hd, g = kv.c.head_dim, kv.c.n_kv
+    check(lib.lrs_rope_append_dev(ctx.h, C.byref(kv.c), C.byref(LrsRope(rope_dim, layout, int(f32_angle), scale)),
+                                  freq.ptr if freq else None, q.ptr, n_head * hd if ldq is None else ldq, k.ptr,
+                                  g * hd if ldk is None else ldk, v.ptr, g * hd if ldv is None else ldv, pos.ptr,
+                                  slot.ptr, n, n_head, q_out.ptr))
+
+
+def tree_mask(parents):
+    """lrs_tree_mask: (mask [n, ceil(n / 32)] u32, depth [n] u32) of a tree of
+    drafted tokens; parents: a node before the child, -1 or NO_PARENT for a root."""
+    p = np.asarray(parents, np.int64) & 0xFFFFFFFF
+    p = np.ascontiguousarray(p, dtype=np.uint32)
+    mask, depth = np.zeros((p.size, (p.size + 31) // 32), np.uint32), np.zeros(p.size, np.uint32)
+    check(lib.lrs_tree_mask(_ptr(p), p.size, _ptr(mask), _ptr(depth)))
+    return mask, depth
+
+
+def attn_tree_dev(ctx: Context, kv: KvCache, q, n: int, n_head: int, length: int, mask, out,
+                  scale: float | None = None) -> None:
+    """lrs_attn_tree_dev (async, device buffers): n tokens over the cache's rows
+    0..length-1 and those of rows length..length+n-1 that mask (None: a chain)
+    lets them see; scale defaults to head_dim^-1/2."""
+    check(lib.lrs_attn_tree_dev(ctx.h, C.byref(kv.c), q.ptr, n, n_head, length, mask.ptr if mask else None,
+                                kv.c.head_dim ** -0.5 if scale is None else scale, out.ptr))
 
 
 class GpuMatmul:

@@ -2,6 +2,8 @@
 #include "gemm_plan.h"
 #include "lrs_internal.h"
 
+#include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -81,7 +83,7 @@ static std::mutex g_scratch_mu;
 static std::unordered_map<lrs_ctx *, lrs_ctx_scratch> g_scratch;
 
 namespace lrs {
-static int ctx_scratch(lrs_ctx *ctx, size_t bytes, void **p, size_t *have = nullptr) {
+int ctx_scratch(lrs_ctx *ctx, size_t bytes, void **p, size_t *have) {
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     lrs_ctx_scratch &s = g_scratch[ctx];
     if (s.n < bytes) {
@@ -574,6 +576,167 @@ int lrs_copy_d2h(lrs_ctx *ctx, void *dst, const void *src_dev, size_t bytes) {
     LRS_HIP(hipStreamSynchronize(ctx->stream));
     return LRS_OK;
 }
+
+}  // extern "C"
+
+// ---- sampled and speculated decoding ----
+namespace lrs {
+int sampling_check(const lrs_sampling *p) {
+    if (!p) return fail(LRS_E_ARG, "null sampling parameters");
+    if (!(p->temperature >= 0.f && p->temperature <= 3.4e38f)) return fail(LRS_E_ARG, "temperature must be finite and >= 0");
+    if (!(p->top_p >= 0.f && p->top_p <= 1.f)) return fail(LRS_E_ARG, "top_p must be in 0..1");
+    if (!(p->min_p >= 0.f && p->min_p <= 1.f)) return fail(LRS_E_ARG, "min_p must be in 0..1");
+    return LRS_OK;
+}
+int tree_check(const uint32_t *parents, uint32_t n) {
+    if (n == 0 || n > LRS_TREE_MAX)
+        return fail(LRS_E_ARG, "a tree has 1 to " + std::to_string(LRS_TREE_MAX) + " nodes");
+    for (uint32_t i = 0; i < n; i++)
+        if (parents[i] != LRS_NO_PARENT && parents[i] >= i)
+            return fail(LRS_E_ARG, "node " + std::to_string(i) + ": its parent must come before it");
+    return LRS_OK;
+}
+int ctx_sample(lrs_ctx *ctx, const float *logits, size_t ld, uint32_t rows, uint32_t vocab, const lrs_sampling *p,
+               const float *u, uint32_t *tok, float *prob, uint32_t *step, uint32_t *gen, uint32_t gen_cap) {
+    void *work = nullptr;
+    if (int rc = ctx_scratch(ctx, sample_work_bytes(rows, vocab, *p), &work)) return rc;
+    LRS_HIP(launch_sample(logits, ld, rows, vocab, *p, u, tok, prob, work, ctx->stream, step, gen, gen_cap));
+    return LRS_OK;
+}
+static int kv_check(const lrs_kv *kv, uint32_t n, uint32_t n_head) {
+    if (!kv || !kv->k || !kv->v) return fail(LRS_E_ARG, "null cache");
+    if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
+        return fail(LRS_E_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+    if (kv->n_kv == 0 || kv->rows == 0 || n == 0) return fail(LRS_E_ARG, "empty dimension");
+    if (kv->rows > 0x7FFFFFFFu) return fail(LRS_E_ARG, "a cache has at most 2^31 - 1 rows");
+    if (n_head == 0 || n_head % kv->n_kv) return fail(LRS_E_ARG, "n_head must be a multiple of n_kv");
+    if (n_head > 1024) return fail(LRS_E_UNSUPPORTED, "more than 1024 heads");
+    if ((uintptr_t)kv->k % 16 || (uintptr_t)kv->v % 16) return fail(LRS_E_ARG, "the cache must be 16-byte aligned");
+    return LRS_OK;
+}
+}  // namespace lrs
+
+extern "C" {
+
+int lrs_sample_dev(lrs_ctx *ctx, const float *logits_dev, size_t ld, uint32_t rows, uint32_t vocab,
+                   const lrs_sampling *p, const float *u_dev, uint32_t *tokens_dev, float *probs_dev) {
+    if (!ctx || !logits_dev || !u_dev || !tokens_dev) return fail(LRS_E_ARG, "null argument");
+    if (int rc = sampling_check(p)) return rc;
+    if (rows == 0 || rows > 65535) return fail(LRS_E_ARG, "rows must be 1..65535");
+    if (vocab == 0 || vocab > LRS_SAMPLE_MAX_VOCAB)
+        return fail(LRS_E_ARG, "vocab must be 1.." + std::to_string(LRS_SAMPLE_MAX_VOCAB));
+    if (ld < vocab) return fail(LRS_E_ARG, "ld is below vocab");
+    SETDEV(ctx);
+    return ctx_sample(ctx, logits_dev, ld, rows, vocab, p, u_dev, tokens_dev, probs_dev, nullptr, nullptr, 0);
+}
+
+int lrs_rope_freqs(uint32_t rope_dim, const lrs_rope_scaling *sc, float *freq, float *scale) {
+    if (!sc || !freq || !scale) return fail(LRS_E_ARG, "null argument");
+    if (rope_dim == 0 || rope_dim % 2 || rope_dim > 256) return fail(LRS_E_ARG, "rope_dim must be even and in 2..256");
+    if (!(sc->base > 1.f) || !std::isfinite(sc->base)) return fail(LRS_E_ARG, "base must be above 1");
+    if (sc->type > LRS_ROPE_YARN) return fail(LRS_E_ARG, "unknown rope scaling type");
+    const double d = rope_dim, b = sc->base, pi2 = 6.283185307179586;
+    if (sc->type != LRS_ROPE_PLAIN && (!(sc->factor >= 1.f) || !std::isfinite(sc->factor)))
+        return fail(LRS_E_ARG, "factor must be at least 1");
+    *scale = 1.f;
+    double lo = 0, hi = 0;
+    if (sc->type == LRS_ROPE_YARN) {
+        if (sc->orig_ctx == 0) return fail(LRS_E_ARG, "orig_ctx must be above 0");
+        if (!(sc->beta_fast > sc->beta_slow && sc->beta_slow > 0.f)) return fail(LRS_E_ARG, "beta_fast > beta_slow > 0");
+        // the pairs that make beta_fast and beta_slow turns over orig_ctx positions
+        auto pair = [&](double turns) { return d * std::log(sc->orig_ctx / (turns * pi2)) / (2.0 * std::log(b)); };
+        lo = std::max(0.0, std::floor(pair(sc->beta_fast)));
+        hi = std::min(d - 1.0, std::ceil(pair(sc->beta_slow)));
+        if (hi <= lo) hi = lo + 0.001;
+        *scale = (float)(0.1 * std::log((double)sc->factor) + 1.0);
+    }
+    for (uint32_t i = 0; i < rope_dim / 2; i++) {
+        double f = std::pow(b, -2.0 * i / d);
+        if (sc->type == LRS_ROPE_LINEAR) f /= sc->factor;
+        if (sc->type == LRS_ROPE_YARN) {
+            const double slow = std::min(1.0, std::max(0.0, (i - lo) / (hi - lo)));
+            f = f * (1.0 - slow) + f / sc->factor * slow;
+        }
+        freq[i] = (float)f;
+    }
+    return LRS_OK;
+}
+
+int lrs_rope_append_dev(lrs_ctx *ctx, const lrs_kv *kv, const lrs_rope *rope, const float *freq_dev, const float *q_dev,
+                        size_t ldq, const float *k_dev, size_t ldk, const float *v_dev, size_t ldv,
+                        const uint32_t *pos_dev, const uint32_t *slot_dev, uint32_t n, uint32_t n_head, float *q_out_dev) {
+    if (!ctx || !rope || !q_dev || !k_dev || !v_dev || !pos_dev || !slot_dev || !q_out_dev)
+        return fail(LRS_E_ARG, "null argument");
+    if (int rc = kv_check(kv, n, n_head)) return rc;
+    if (n > 65535) return fail(LRS_E_ARG, "n must be at most 65535");
+    if (rope->rope_dim % 2 || rope->rope_dim > kv->head_dim) return fail(LRS_E_ARG, "bad rope_dim");
+    if (rope->rope_dim && !freq_dev) return fail(LRS_E_ARG, "null freq");
+    if (rope->layout != LRS_ROPE_PAIRS && rope->layout != LRS_ROPE_HALVES) return fail(LRS_E_ARG, "unknown rope layout");
+    if (!std::isfinite(rope->scale)) return fail(LRS_E_ARG, "scale must be finite");
+    const size_t qd = (size_t)n_head * kv->head_dim, kvd = (size_t)kv->n_kv * kv->head_dim;
+    if (ldq < qd || ldk < kvd || ldv < kvd) return fail(LRS_E_ARG, "a row stride is below its row");
+    if (q_out_dev == q_dev && ldq != qd) return fail(LRS_E_ARG, "q_out may be q only where q's rows are dense");
+    SETDEV(ctx);
+    RopeAppend a = {};
+    a.q = q_dev, a.k = k_dev, a.v = v_dev;
+    a.ldq = ldq, a.ldk = ldk, a.ldv = ldv;
+    a.freq = freq_dev;
+    a.pos = pos_dev, a.slot = slot_dev;
+    a.q_out = q_out_dev;
+    a.kc = (_Float16 *)kv->k, a.vc = (_Float16 *)kv->v;
+    a.n = n, a.n_head = n_head, a.n_kv = kv->n_kv, a.head_dim = kv->head_dim, a.rows = kv->rows;
+    a.rope_dim = rope->rope_dim;
+    a.halves = rope->layout == LRS_ROPE_HALVES;
+    a.f32_angle = rope->f32_angle != 0;
+    a.scale = rope->scale;
+    LRS_HIP(launch_rope_append(a, ctx->stream));
+    return LRS_OK;
+}
+
+int lrs_tree_mask(const uint32_t *parents, uint32_t n, uint32_t *mask, uint32_t *depth) {
+    if (!parents || !mask) return fail(LRS_E_ARG, "null argument");
+    if (int rc = tree_check(parents, n)) return rc;
+    const uint32_t W = (n + 31) / 32;
+    for (uint32_t i = 0; i < n; i++) {
+        uint32_t *const m = mask + (size_t)i * W;
+        if (parents[i] == LRS_NO_PARENT)
+            memset(m, 0, 4 * W);
+        else
+            memcpy(m, mask + (size_t)parents[i] * W, 4 * W);
+        m[i / 32] |= 1u << (i % 32);
+        if (depth) depth[i] = parents[i] == LRS_NO_PARENT ? 0 : depth[parents[i]] + 1;
+    }
+    return LRS_OK;
+}
+
+int lrs_attn_tree_dev(lrs_ctx *ctx, const lrs_kv *kv, const float *q_dev, uint32_t n, uint32_t n_head, uint32_t len,
+                      const uint32_t *mask_dev, float scale, float *out_dev) {
+    if (!ctx || !q_dev || !out_dev) return fail(LRS_E_ARG, "null argument");
+    if (int rc = kv_check(kv, n, n_head)) return rc;
+    if (n > LRS_TREE_MAX) return fail(LRS_E_ARG, "n must be at most " + std::to_string(LRS_TREE_MAX));
+    if ((uint64_t)len + n > kv->rows) return fail(LRS_E_CTX_OVERFLOW, "len + n exceeds the cache");
+    if (!std::isfinite(scale)) return fail(LRS_E_ARG, "scale must be finite");
+    if ((uintptr_t)q_dev % 16 || (uintptr_t)out_dev % 16) return fail(LRS_E_ARG, "q and out must be 16-byte aligned");
+    if (q_dev == out_dev) return fail(LRS_E_ARG, "out must not be the same buffer as q");
+    SETDEV(ctx);
+    void *work = nullptr;
+    const size_t wb = attn_tree_work_bytes(n, len, n_head, kv->n_kv, kv->head_dim);
+    if (wb)
+        if (int rc = ctx_scratch(ctx, wb, &work)) return rc;
+    AttnTree a = {};
+    a.q = q_dev;
+    a.kc = (const _Float16 *)kv->k, a.vc = (const _Float16 *)kv->v;
+    a.mask = mask_dev;
+    a.out = out_dev;
+    a.n = n, a.len = len, a.n_head = n_head, a.n_kv = kv->n_kv, a.rows = kv->rows;
+    a.scale = scale;
+    LRS_HIP(launch_attn_tree(a, kv->head_dim, work, ctx->stream));
+    return LRS_OK;
+}
+
+}  // extern "C"
+
+extern "C" {
 
 // ---- graph capture of the asynchronous (*_dev) entry points ----
 struct lrs_graph {

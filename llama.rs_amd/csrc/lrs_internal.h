@@ -181,6 +181,56 @@ hipError_t launch_attn_prefill(const float *q, const _Float16 *kc, const _Float1
 // silu(G) * U [n][F] as a GEMM input of precision 3; F a multiple of 256
 hipError_t launch_swiglu_pack(const float *G, const float *U, uint32_t F, uint32_t n, uint8_t *planes,
                               hipStream_t s);
+// sampling (sample.hip): a row's token (and, row 0, the next step's words: step
+// {token, pos, n}, gen[n]) from its logits and u[row]; work: sample_work_bytes
+size_t sample_work_bytes(uint32_t rows, uint32_t vocab, const lrs_sampling &p);
+hipError_t launch_sample(const float *x, size_t ld, uint32_t rows, uint32_t vocab, const lrs_sampling &p, const float *u,
+                         uint32_t *tok, float *prob, void *work, hipStream_t s, uint32_t *step = nullptr,
+                         uint32_t *gen = nullptr, uint32_t gen_cap = 0);
+// a tree of drafted tokens (tree.hip)
+struct RopeAppend {
+    const float *q, *k, *v;        // rows of ldq, ldk, ldv floats
+    size_t ldq, ldk, ldv;
+    const float *bq, *bk, *bv;     // added first; or null
+    const float *freq;             // [rope_dim / 2]
+    const uint32_t *pos, *slot;    // [n]; a slot past the cache stores nothing
+    float *q_out;                  // [n][n_head * head_dim]; may be q
+    _Float16 *kc, *vc;             // [n_kv][rows][head_dim]
+    uint32_t n, n_head, n_kv, head_dim, rows, rope_dim;
+    int halves, f32_angle;         // pairs (i, i + rope_dim / 2); angles rounded to f32
+    float scale;
+};
+hipError_t launch_rope_append(const RopeAppend &a, hipStream_t s);
+struct AttnTree {
+    const float *q;                // [n][n_head * hd]
+    const _Float16 *kc, *vc;       // [n_kv][rows][hd]
+    const uint32_t *mask;          // [n][ceil(n / 32)], or null: node i sees nodes 0..i
+    float *out;                    // [n][n_head * hd]
+    uint32_t n, len, n_head, n_kv, rows;
+    float scale;
+    // set by the launch: row tiles, shares of the positions, their sums
+    uint32_t tiles, S;
+    float *part;                   // [S][n][n_head * hd]
+    float2 *ml;                    // [S][n][n_head]: {maximum (of powers of two), sum}
+};
+constexpr size_t TREE_WORK = 8u << 20;  // attn_tree_work_bytes is never above
+uint32_t attn_tree_splits(uint32_t n, uint32_t len, uint32_t n_head, uint32_t n_kv, uint32_t hd);
+size_t attn_tree_work_bytes(uint32_t n, uint32_t len, uint32_t n_head, uint32_t n_kv, uint32_t hd);
+hipError_t launch_attn_tree(AttnTree a, uint32_t hd, void *work, hipStream_t s);
+// out: {length, sampled tokens} of the walk from node 0, path: its nodes
+hipError_t launch_tree_walk(const uint32_t *tokens, const uint32_t *parents, const uint32_t *sampled, uint32_t n,
+                            uint32_t *out, uint32_t *path, hipStream_t s);
+// rows pos0 + path[i] to pos0 + i, i < *count, of `planes` caches [ctx][hd]
+hipError_t launch_kv_keep(_Float16 *kv, uint32_t planes, uint32_t hd, uint32_t ctx, uint32_t pos0, const uint32_t *count,
+                          const uint32_t *path, hipStream_t s);
+// argument checks shared by the kernel-level and the model's entry points
+int sampling_check(const lrs_sampling *p);
+int tree_check(const uint32_t *parents, uint32_t n);
+// lrs_sample_dev's launches in the context's scratch, the step's words written too
+int ctx_sample(lrs_ctx *ctx, const float *logits, size_t ld, uint32_t rows, uint32_t vocab, const lrs_sampling *p,
+               const float *u, uint32_t *tok, float *prob, uint32_t *step, uint32_t *gen, uint32_t gen_cap);
+// the context's scratch, at least `bytes` of it
+int ctx_scratch(lrs_ctx *ctx, size_t bytes, void **p, size_t *have = nullptr);
 // hybrid (qwen35) mixers (dn.hip)
 // QK-norm + RoPE of the hybrid's gated attention run by the split kernel
 // (attention.hip, QP): query rows from the projection's q + gate rows, the

@@ -211,6 +211,18 @@ struct lrs_model {
     size_t rec_bytes = 0;
     // weights the model owns (built by lrs_model_load_gguf), freed with it
     std::vector<lrs_weight *> owned;
+    // sampling: one random number per token of a call, the sampler's workspace
+    float *u_dev = nullptr;
+    void *samp = nullptr;
+    size_t samp_bytes = 0;
+    // a tree of drafted tokens: its words on the host (pinned) and the device
+    // (tree_words), the attention's partial sums, every node's logits and
+    // sampled token, {length, tokens} of the walk, its nodes
+    uint32_t *tree_host = nullptr, *tree_dev = nullptr, *tree_out = nullptr, *tree_path = nullptr, *tree_tok = nullptr;
+    void *tree_work = nullptr;
+    void *tree_logits = nullptr;
+    size_t tree_logits_bytes = 0;
+    uint32_t tree_n = 0, tree_pos0 = 0;  // the tree that lrs_tree_keep may keep (n 0: none)
 };
 
 // hands the loader's uploaded weights to the model
@@ -1184,6 +1196,9 @@ void lrs_model_destroy(lrs_model *m) {
     if (m->words_host) (void)hipHostFree(m->words_host);
     if (m->logits_host) (void)hipHostFree(m->logits_host);
     if (m->gen_host) (void)hipHostFree(m->gen_host);
+    if (m->tree_host) (void)hipHostFree(m->tree_host);
+    if (m->samp) (void)hipFree(m->samp);
+    if (m->tree_logits) (void)hipFree(m->tree_logits);
     for (lrs_weight *w : m->owned) lrs_weight_free(w);
     delete m;
 }
@@ -1358,7 +1373,12 @@ static int ensure_prefill(lrs_model *m) {
 
 // one block of nb tokens at positions pos0.. through every layer (the
 // forward of model.rs:99-266 with the matmuls as GEMMs of precision 3); leaves the residual rows in pX
-static int prefill_block(lrs_model *m, const uint32_t *tokens, uint32_t nb, uint32_t pos0) {
+// (tree: a block of drafted tokens with positions, slots and a mask of their own,
+// dense models)
+struct TreeStep {
+    const uint32_t *pos, *slot, *mask;
+};
+static int prefill_block(lrs_model *m, const uint32_t *tokens, uint32_t nb, uint32_t pos0, const TreeStep *tree = nullptr) {
     const lrs_config &c = m->cfg;
     hipStream_t s = m->ctx->stream;
     const uint32_t qd = c.n_head * c.head_dim, kvd = c.n_head_kv * c.head_dim, E = c.n_embd;
@@ -1492,6 +1512,33 @@ static int prefill_block(lrs_model *m, const uint32_t *tokens, uint32_t nb, uint
             const uint32_t N[3] = {qd, kvd, kvd};
             LRS_HIP(gemm_group(3, w, y, N));
         }
+        if (tree) {
+            RopeAppend ra = {};
+            ra.q = m->pQt, ra.k = m->pKt, ra.v = m->pVt;
+            ra.ldq = qd, ra.ldk = kvd, ra.ldv = kvd;
+            ra.bq = L.bq, ra.bk = L.bk, ra.bv = L.bv;
+            ra.freq = m->freq;
+            ra.pos = tree->pos, ra.slot = tree->slot;
+            ra.q_out = m->pQ;
+            ra.kc = L.kc, ra.vc = L.vc;
+            ra.n = nb, ra.n_head = c.n_head, ra.n_kv = c.n_head_kv, ra.head_dim = c.head_dim, ra.rows = c.ctx;
+            ra.rope_dim = c.rope_dim;
+            ra.f32_angle = 1;  // a key has the same angle however it entered the cache
+            ra.scale = 1.0f;
+            LRS_HIP(launch_rope_append(ra, s));
+            AttnTree at = {};
+            at.q = m->pQ;
+            at.kc = L.kc, at.vc = L.vc;
+            at.mask = tree->mask;
+            at.out = m->pATT;
+            at.n = nb, at.len = pos0, at.n_head = c.n_head, at.n_kv = c.n_head_kv, at.rows = c.ctx;
+            at.scale = 1.0f / sqrtf((float)c.head_dim);
+            LRS_HIP(launch_attn_tree(at, c.head_dim, m->tree_work, s));
+            LRS_HIP(pack(m->pATT, qd));
+            LRS_HIP(gemm_resid_norm(L.o, L.ffn_norm, nullptr));
+            LRS_HIP(ffn(l));
+            continue;
+        }
         LRS_HIP(launch_qkv_post(m->pQt, m->pKt, m->pVt, L.bq, L.bk, L.bv, m->freq, m->pQ, L.kc,
                                 L.vc, nb, pos0, qd, kvd, c.head_dim, c.rope_dim, c.ctx, s));
         LRS_HIP(launch_attn_prefill(m->pQ, L.kc, L.vc, nullptr, m->pATT, m->pML, nb, pos0, c.n_head,
@@ -1541,6 +1588,7 @@ int lrs_decode(lrs_model *m, uint32_t token, uint32_t pos, float *logits) {
     if (!m || !logits) return fail(LRS_E_ARG, "null argument");
     int rc = check_step(m, token, pos);
     if (rc || (rc = check_continue(m, pos))) return rc;
+    m->tree_n = 0;
     LRS_HIP(hipSetDevice(m->ctx->device));
     hipStream_t s = m->ctx->stream;
     LRS_HIP(set_step(m, token, pos));
@@ -1566,6 +1614,7 @@ int lrs_decode_batch(lrs_model *m, const uint32_t *tokens, uint32_t n, uint32_t 
     // every weight has one, else token by token
     int rc = check_continue(m, pos0);
     if (rc) return rc;
+    m->tree_n = 0;
     if (n > 1 && prefill_capable(m)) {
         for (uint32_t i = 0; i < n; i++)
             if ((rc = check_step(m, tokens[i], pos0 + i))) return rc;
@@ -1587,6 +1636,7 @@ int lrs_decode_batch(lrs_model *m, const uint32_t *tokens, uint32_t n, uint32_t 
 void lrs_reset(lrs_model *m) {
     if (!m) return;
     m->len = 0;
+    m->tree_n = 0;
     if (m->rec) {
         // delta-net states and conv windows back to zero (the KV cache needs
         // no clearing: attention reads positions 0..pos only)
@@ -1611,6 +1661,7 @@ int lrs_decode_greedy(lrs_model *m, uint32_t token, uint32_t pos, uint32_t *next
     if (!m || !next) return fail(LRS_E_ARG, "null argument");
     int rc = check_step(m, token, pos);
     if (rc || (rc = check_continue(m, pos))) return rc;
+    m->tree_n = 0;
     LRS_HIP(hipSetDevice(m->ctx->device));
     hipStream_t s = m->ctx->stream;
     LRS_HIP(set_step(m, token, pos));
@@ -1623,10 +1674,34 @@ int lrs_decode_greedy(lrs_model *m, uint32_t token, uint32_t pos, uint32_t *next
     return LRS_OK;
 }
 
-int lrs_generate_greedy(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uint32_t pos0,
-                        uint32_t n_gen, uint32_t *out_tokens) {
-    if (!m || !prompt || !out_tokens || n_prompt == 0 || n_gen == 0)
-        return fail(LRS_E_ARG, "null argument / empty prompt or generation");
+// the sampler's workspace and the random numbers of a call of n tokens over rows
+// of logits; these buffers are in no captured graph
+static int grow(lrs_model *m, void **p, size_t *have, size_t bytes) {
+    if (*have >= bytes) return LRS_OK;
+    LRS_HIP(hipStreamSynchronize(m->ctx->stream));
+    if (*p) (void)hipFree(*p);
+    *p = nullptr;
+    *have = 0;
+    const hipError_t e = hipMalloc(p, bytes);
+    if (e != hipSuccess) return hip_fail(e, "hipMalloc(model)");
+    *have = bytes;
+    return LRS_OK;
+}
+static int ensure_sample(lrs_model *m, const lrs_sampling *p, uint32_t rows) {
+    if (m->cfg.vocab > LRS_SAMPLE_MAX_VOCAB) return fail(LRS_E_UNSUPPORTED, "vocabulary too large to sample");
+    if (!m->u_dev)
+        if (int rc = dev_alloc(m, m->gen_cap * sizeof(float), (void **)&m->u_dev)) return rc;
+    return grow(m, &m->samp, &m->samp_bytes, sample_work_bytes(rows, m->cfg.vocab, *p));
+}
+// the token of the forward just enqueued, from u_dev[i]; the next step's words too
+static hipError_t sample_step(lrs_model *m, const lrs_sampling *p, uint32_t i) {
+    return launch_sample(m->logits, m->cfg.vocab, 1, m->cfg.vocab, *p, m->u_dev + i, m->step + 3, nullptr, m->samp,
+                         m->ctx->stream, m->step, m->gen, m->gen_cap);
+}
+
+// prompt, then n_gen tokens that are greedy (p null) or sampled from u
+static int generate(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uint32_t pos0, uint32_t n_gen,
+                    const lrs_sampling *p, const float *u, uint32_t *out_tokens) {
     // the last generated token is not fed back, so it needs no cache slot
     if ((size_t)pos0 + n_prompt + n_gen - 1 > m->cfg.ctx)
         return fail(LRS_E_CTX_OVERFLOW, "prompt + generation exceed the context");
@@ -1634,24 +1709,212 @@ int lrs_generate_greedy(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt,
     for (uint32_t i = 0; i < n_prompt; i++)
         if (prompt[i] >= m->cfg.vocab) return fail(LRS_E_ARG, "prompt token outside the vocabulary");
     if (int rc0 = check_continue(m, pos0)) return rc0;
+    m->tree_n = 0;
     LRS_HIP(hipSetDevice(m->ctx->device));
     hipStream_t s = m->ctx->stream;
     // prefill: tokens 0..n_prompt-2, then the last prompt token starts the
-    // greedy chain (its argmax is the first generated token)
+    // chain (the token after it is the first generated one)
     int rc = LRS_OK;
+    if (p) {
+        if ((rc = ensure_sample(m, p, 1))) return rc;
+        LRS_HIP(hipMemcpyAsync(m->u_dev, u, n_gen * sizeof(float), hipMemcpyHostToDevice, s));
+    }
     if (n_prompt > 2 && prefill_capable(m)) {
         if ((rc = prefill(m, prompt, n_prompt - 1, pos0, false))) return rc;
     } else if (n_prompt > 1 && (rc = enqueue_tokens(m, prompt, n_prompt - 1, pos0))) {
         return rc;
     }
     LRS_HIP(set_step(m, prompt[n_prompt - 1], pos0 + n_prompt - 1));
-    for (uint32_t i = 0; i < n_gen; i++) LRS_HIP(run_forward(m, true));
+    for (uint32_t i = 0; i < n_gen; i++) {
+        LRS_HIP(run_forward(m, !p));
+        if (p) LRS_HIP(sample_step(m, p, i));
+    }
     // through the pinned buffer: the caller's memory is pageable
     LRS_HIP(publish(m, m->gen, m->gen_host, n_gen));
     LRS_HIP(hipStreamSynchronize(s));
     if (int e = ao_err_check(m)) return e;
     memcpy(out_tokens, m->gen_host, n_gen * sizeof(uint32_t));
+    if (p)
+        for (uint32_t i = 0; i < n_gen; i++)
+            if (out_tokens[i] == LRS_NO_TOKEN) return fail(LRS_E_HIP, "no word of the logits can be sampled");
     m->len = pos0 + n_prompt + n_gen - 1;
+    return LRS_OK;
+}
+
+int lrs_generate_greedy(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uint32_t pos0,
+                        uint32_t n_gen, uint32_t *out_tokens) {
+    if (!m || !prompt || !out_tokens || n_prompt == 0 || n_gen == 0)
+        return fail(LRS_E_ARG, "null argument / empty prompt or generation");
+    return generate(m, prompt, n_prompt, pos0, n_gen, nullptr, nullptr, out_tokens);
+}
+
+int lrs_generate_sample(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uint32_t pos0, uint32_t n_gen,
+                        const lrs_sampling *p, const float *u, uint32_t *out_tokens) {
+    if (!m || !prompt || !u || !out_tokens || n_prompt == 0 || n_gen == 0)
+        return fail(LRS_E_ARG, "null argument / empty prompt or generation");
+    if (int rc = sampling_check(p)) return rc;
+    return generate(m, prompt, n_prompt, pos0, n_gen, p, u, out_tokens);
+}
+
+__global__ void k_set_u(float *u_dev, float u) { *u_dev = u; }
+
+int lrs_decode_sample(lrs_model *m, uint32_t token, uint32_t pos, const lrs_sampling *p, float u, uint32_t *next) {
+    if (!m || !next) return fail(LRS_E_ARG, "null argument");
+    int rc = sampling_check(p);
+    if (rc || (rc = check_step(m, token, pos)) || (rc = check_continue(m, pos))) return rc;
+    m->tree_n = 0;
+    LRS_HIP(hipSetDevice(m->ctx->device));
+    hipStream_t s = m->ctx->stream;
+    if ((rc = ensure_sample(m, p, 1))) return rc;
+    LRS_HIP(set_step(m, token, pos));
+    LRS_HIP(run_forward(m, false));
+    hipLaunchKernelGGL(k_set_u, dim3(1), dim3(1), 0, s, m->u_dev, u);
+    LRS_HIP(sample_step(m, p, 0));
+    LRS_HIP(publish(m, m->step, m->words_host, 1));
+    LRS_HIP(hipStreamSynchronize(s));
+    if (int e = ao_err_check(m)) return e;
+    if (m->words_host[0] == LRS_NO_TOKEN) return fail(LRS_E_HIP, "no word of the logits can be sampled");
+    *next = m->words_host[0];
+    m->len = pos + 1;
+    return LRS_OK;
+}
+
+// ---- trees of drafted tokens ----
+// words of a tree of n nodes, in tree_host and tree_dev: token, position, slot,
+// parent and random number of each, then the mask
+static constexpr size_t TREE_WORDS = 5 * LRS_TREE_MAX + LRS_TREE_MAX * (LRS_TREE_MAX / 32);
+static_assert(LRS_TREE_MAX <= PREFILL_BLOCK, "a tree is one prompt block");
+
+static int ensure_tree(lrs_model *m, uint32_t n) {
+    if (int rc = ensure_prefill(m)) return rc;
+    if (!m->tree_host) {
+        int rc;
+        if ((!m->tree_dev && (rc = dev_alloc(m, TREE_WORDS * 4, (void **)&m->tree_dev))) ||
+            (!m->tree_tok && (rc = dev_alloc(m, LRS_TREE_MAX * 4, (void **)&m->tree_tok))) ||
+            (!m->tree_out && (rc = dev_alloc(m, (LRS_TREE_MAX + 4) * 4, (void **)&m->tree_out))) ||
+            (!m->tree_path && (rc = dev_alloc(m, (LRS_TREE_MAX + 4) * 4, (void **)&m->tree_path))) ||
+            (!m->tree_work && (rc = dev_alloc(m, TREE_WORK, &m->tree_work))))
+            return rc;
+        if (hipHostMalloc((void **)&m->tree_host, TREE_WORDS * 4, hipHostMallocDefault) != hipSuccess) {
+            m->tree_host = nullptr;
+            return fail(LRS_E_OOM, "pinned host buffers");
+        }
+    }
+    return grow(m, &m->tree_logits, &m->tree_logits_bytes, (size_t)n * m->cfg.vocab * sizeof(float));
+}
+
+static int tree_args(lrs_model *m, const uint32_t *tokens, const uint32_t *parents, uint32_t n, uint32_t pos0) {
+    if (m->hybrid)
+        return fail(LRS_E_UNSUPPORTED, "trees need a dense model (a recurrent state follows one sequence)");
+    if (m->head_q8 || !prefill_capable(m)) return fail(LRS_E_UNSUPPORTED, "trees need a model with prompt blocks");
+    if (int rc = tree_check(parents, n)) return rc;
+    if ((size_t)pos0 + n > m->cfg.ctx)
+        return fail(LRS_E_CTX_OVERFLOW, "position " + std::to_string(pos0) + " + " + std::to_string(n) +
+                                            " nodes exceed the context");
+    for (uint32_t i = 0; i < n; i++)
+        if (tokens[i] >= m->cfg.vocab)
+            return fail(LRS_E_ARG, "token " + std::to_string(tokens[i]) + " outside the vocabulary");
+    return LRS_OK;
+}
+
+// enqueues the tree's forward: every node's logits in tree_logits
+static int tree_forward(lrs_model *m, const uint32_t *tokens, const uint32_t *parents, uint32_t n, uint32_t pos0,
+                        const float *u) {
+    hipStream_t s = m->ctx->stream;
+    const lrs_config &c = m->cfg;
+    m->tree_n = 0;
+    m->len = std::min(m->len, pos0);  // the rows behind pos0 are overwritten
+    if (int rc = ensure_tree(m, n)) return rc;
+    LRS_HIP(hipStreamSynchronize(s));  // a call before may still read the pinned words
+    uint32_t *const w = m->tree_host;
+    const uint32_t W = (n + 31) / 32, words = 5 * n + n * W;
+    memcpy(w, tokens, n * 4);
+    memcpy(w + 3 * n, parents, n * 4);
+    if (u)
+        memcpy(w + 4 * n, u, n * 4);
+    else
+        memset(w + 4 * n, 0, n * 4);
+    if (int rc = lrs_tree_mask(parents, n, w + 5 * n, w + n)) return rc;
+    for (uint32_t i = 0; i < n; i++) {
+        w[n + i] += pos0;
+        w[2 * n + i] = pos0 + i;
+    }
+    LRS_HIP(launch_copy_words(w, words, m->tree_dev, s));
+    const TreeStep t = {m->tree_dev + n, m->tree_dev + 2 * n, m->tree_dev + 5 * n};
+    if (int rc = prefill_block(m, tokens, n, pos0, &t)) return rc;
+    LRS_HIP(launch_norm_rows(nullptr, 0, m->pX, m->output_norm, c.rms_eps, c.n_embd, n, nullptr, m->pA, s));
+    float *const y = (float *)m->tree_logits;
+    LRS_HIP(launch_gemm_segs(&m->output->v, &y, &c.vocab, 1, m->pA, n, 3, s, false, m->pWork, m->work_bytes));
+    m->len = pos0;
+    return LRS_OK;
+}
+
+static hipError_t keep_rows(lrs_model *m, uint32_t pos0) {
+    const lrs_config &c = m->cfg;
+    return launch_kv_keep(m->kv, c.n_layer * 2 * c.n_head_kv, c.head_dim, c.ctx, pos0, m->tree_out, m->tree_path, m->ctx->stream);
+}
+
+int lrs_decode_tree(lrs_model *m, const uint32_t *tokens, const uint32_t *parents, uint32_t n, uint32_t pos0,
+                    float *logits) {
+    if (!m || !tokens || !parents) return fail(LRS_E_ARG, "null argument");
+    int rc = tree_args(m, tokens, parents, n, pos0);
+    if (rc) return rc;
+    LRS_HIP(hipSetDevice(m->ctx->device));
+    if ((rc = tree_forward(m, tokens, parents, n, pos0, nullptr))) return rc;
+    if (logits)
+        LRS_HIP(hipMemcpyAsync(logits, m->tree_logits, (size_t)n * m->cfg.vocab * sizeof(float), hipMemcpyDeviceToHost,
+                               m->ctx->stream));
+    LRS_HIP(hipStreamSynchronize(m->ctx->stream));
+    m->tree_n = n;
+    m->tree_pos0 = pos0;
+    return LRS_OK;
+}
+
+int lrs_tree_keep(lrs_model *m, const uint32_t *nodes, uint32_t n_nodes) {
+    if (!m || !nodes) return fail(LRS_E_ARG, "null argument");
+    if (m->tree_n == 0) return fail(LRS_E_ARG, "no tree to keep nodes of");
+    if (n_nodes == 0 || n_nodes > m->tree_n) return fail(LRS_E_ARG, "bad number of nodes");
+    const uint32_t *const parents = m->tree_host + 3 * m->tree_n;
+    for (uint32_t i = 0; i < n_nodes; i++)
+        if (nodes[i] >= m->tree_n || parents[nodes[i]] != (i ? nodes[i - 1] : LRS_NO_PARENT))
+            return fail(LRS_E_ARG, "nodes must be a path of the tree from a root down");
+    LRS_HIP(hipSetDevice(m->ctx->device));
+    hipStream_t s = m->ctx->stream;
+    // behind the parents, which stay for the checks: the call before has synchronised
+    uint32_t *const w = m->tree_host + 5 * LRS_TREE_MAX;
+    memcpy(w, nodes, n_nodes * 4);
+    LRS_HIP(launch_copy_words(w, n_nodes, m->tree_path, s));
+    hipLaunchKernelGGL(k_set_step, dim3(1), dim3(1), 0, s, m->tree_out, n_nodes, 0u);
+    LRS_HIP(keep_rows(m, m->tree_pos0));
+    LRS_HIP(hipStreamSynchronize(s));
+    m->len = m->tree_pos0 + n_nodes;
+    m->tree_n = 0;
+    return LRS_OK;
+}
+
+int lrs_verify_tree(lrs_model *m, const uint32_t *tokens, const uint32_t *parents, uint32_t n, uint32_t pos0,
+                    const lrs_sampling *p, const float *u, uint32_t *out_tokens, uint32_t *n_out) {
+    if (!m || !tokens || !parents || !out_tokens || !n_out) return fail(LRS_E_ARG, "null argument");
+    int rc = sampling_check(p);
+    if (rc || (rc = tree_args(m, tokens, parents, n, pos0))) return rc;
+    if (!u && p->temperature != 0.f) return fail(LRS_E_ARG, "u may be NULL at temperature 0 only");
+    for (uint32_t i = 1; i < n; i++)
+        if (parents[i] == LRS_NO_PARENT) return fail(LRS_E_ARG, "node 0 must be the tree's only root");
+    LRS_HIP(hipSetDevice(m->ctx->device));
+    hipStream_t s = m->ctx->stream;
+    if ((rc = ensure_sample(m, p, n)) || (rc = tree_forward(m, tokens, parents, n, pos0, u))) return rc;
+    LRS_HIP(launch_sample((const float *)m->tree_logits, m->cfg.vocab, n, m->cfg.vocab, *p,
+                          reinterpret_cast<const float *>(m->tree_dev + 4 * n), m->tree_tok, nullptr, m->samp, s));
+    LRS_HIP(launch_tree_walk(m->tree_dev, m->tree_dev + 3 * n, m->tree_tok, n, m->tree_out, m->tree_path, s));
+    LRS_HIP(keep_rows(m, pos0));
+    LRS_HIP(publish(m, m->tree_out, m->tree_host, n + 1));
+    LRS_HIP(hipStreamSynchronize(s));
+    const uint32_t k = m->tree_host[0];
+    for (uint32_t i = 0; i < k; i++)
+        if (m->tree_host[1 + i] == LRS_NO_TOKEN) return fail(LRS_E_HIP, "no word of the logits can be sampled");
+    memcpy(out_tokens, m->tree_host + 1, k * 4);
+    *n_out = k;
+    m->len = pos0 + k;
     return LRS_OK;
 }
 

@@ -1,0 +1,783 @@
+// sample.hip — one token of each row of logits from a given random number:
+// temperature, top-k, top-p, min-p (Sampler::sample, llama-sampling/src/
+// sampler.rs:24-88, does the first three on the host).
+//
+// The order of a row's words is logit descending, index ascending; weights are
+// w_i = e^((l_i - l_max) / T).  The kept set is a prefix of that order:
+//   K  the first top_k words (0: all)
+//   P  the shortest prefix of K whose weights sum to at least top_p times K's
+//   M  the words of P with w >= min_p
+// and the token is the least index i of M with sum_{j in M, j <= i} w_j > u S,
+// S = sum_M w: the inverse of the distribution function in index order, which
+// needs no sorted copy of the row.  NaN counts as -inf and is never taken.
+//
+// A word is one 64-bit value, ordered as the row is: the logit's bits made
+// monotone, then the complement of its index, so that no two are equal and ties
+// go to the lower index.  Weights are whole multiples of 2^-42 (of the largest
+// word's weight) in 64 bits: their sums do not depend on the order in which
+// atomics or wavefronts add them, 2^21 words cannot overflow them, and a sum is
+// off by less than 2^-43 per word.  exp is evaluated in double: the cuts and the
+// token depend on sums next to a border, where 2^-24 of a sum is many words.
+//
+// Two forms.  top_k up to TK (greedy rows among them: top_k = 1): each
+// workgroup selects the top_k of its part of a row (k_part), one workgroup per
+// row merges the parts and picks (k_pick).  Otherwise: the row's range (k_range),
+// a histogram of 2048 bins over it (k_hist), the words of the bins in which the
+// cuts fall and the sums of the parts above (k_collect), the cuts and the token
+// (k_finish).
+#include "lrs_internal.h"
+
+namespace lrs {
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr uint32_t TK = 128;        // top_k of the first form
+constexpr uint32_t PICK_MAX = 8192; // words that a row's parts give it at most
+constexpr uint32_t NB = 2048;       // bins of the second form
+constexpr uint32_t LIST = 2048;     // words of the cuts' bins kept per row
+constexpr uint32_t MAX_PARTS = 256;
+constexpr double ONE = 4398046511104.0;  // 2^42
+
+struct Row {
+    const float *x;
+    size_t ld;
+    uint32_t vocab, parts, part;  // part: words per workgroup (second form)
+    double inv_t;
+    float top_p, min_p, temp;
+    uint32_t k;  // 0: all
+    const float *u;
+    uint32_t *tok;
+    float *prob;           // or null
+    uint32_t *step, *gen;  // the token as the next step's too (row 0), or null
+    uint32_t gen_cap;
+    bool vec;  // rows are 16-byte aligned
+};
+
+// the logit as an unsigned number of the same order; 0: never taken
+__device__ __forceinline__ uint32_t ord(float l) {
+    const float z = l + 0.0f;  // -0 and 0 tie
+    if (!(z > -INFINITY)) return 0u;
+    const uint32_t b = __float_as_uint(z);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unord(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ u64 word(float l, uint32_t i) {
+    const uint32_t k = ord(l);
+    return k ? (u64)k << 32 | (0xFFFFFFFFu - i) : 0ull;
+}
+__device__ __forceinline__ uint32_t word_index(u64 w) { return 0xFFFFFFFFu - (uint32_t)w; }
+__device__ __forceinline__ float word_logit(u64 w) { return unord((uint32_t)(w >> 32)); }
+
+// e^((l - top) / T), 1 for the top's equals (an infinite top leaves the rest nothing)
+__device__ __forceinline__ double weight(float l, float top, double inv_t) {
+    return l == top ? 1.0 : exp(((double)l - (double)top) * inv_t);
+}
+__device__ __forceinline__ u64 fixed(double w) { return (u64)(w * ONE + 0.5); }
+
+// l[0..4) of elements i.. of a row, -inf past its end
+__device__ __forceinline__ void load4(const Row &a, const float *x, uint32_t i, float (&l)[4]) {
+    if (a.vec && i + 4 <= a.vocab) {
+        const float4 v = *reinterpret_cast<const float4 *>(x + i);
+        l[0] = v.x, l[1] = v.y, l[2] = v.z, l[3] = v.w;
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) l[j] = i + j < a.vocab ? x[i + j] : -INFINITY;
+    }
+}
+
+__device__ __forceinline__ double row_u(const Row &a, uint32_t row) {
+    const float u = a.u[row];
+    return u > 0.f ? (double)u : 0.0;
+}
+
+__device__ __forceinline__ void emit(const Row &a, uint32_t row, uint32_t tok, float p) {
+    a.tok[row] = tok;
+    if (a.prob) a.prob[row] = p;
+    if (a.step && row == 0) {
+        const uint32_t n = a.step[2];
+        if (a.gen && n < a.gen_cap) a.gen[n] = tok;
+        a.step[0] = tok;
+        a.step[1] = a.step[1] + 1;
+        a.step[2] = n + 1;
+    }
+}
+
+// ---- top_k up to TK -------------------------------------------------------
+// The top_k words of a part (pieces g, g + parts, .. of 1024 words), descending,
+// zeros behind them.  The k-th largest of the 256 threads' own maxima bounds
+// them from below, so that of a part's words little more than k are ranked
+// against one another, at most k threads' all.
+template <int E>
+__global__ __launch_bounds__(256) void k_part(Row a, u64 *__restrict__ out) {
+    __shared__ __attribute__((aligned(16))) u64 best[256];
+    __shared__ __attribute__((aligned(16))) u64 list[4 * E * TK];
+    __shared__ u64 thr;
+    __shared__ uint32_t cnt;
+    const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y, k = a.k;
+    const float *const x = a.x + row * a.ld;
+    float l[E][4];
+    u64 m = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const size_t i = ((size_t)g + (size_t)a.parts * e) * 1024 + 4 * tid;
+        load4(a, x, (uint32_t)min(i, (size_t)a.vocab), l[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const uint32_t i = (g + a.parts * e) * 1024 + 4 * tid;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) m = max(m, word(l[e][j], i + j));
+    }
+    best[tid] = m;
+    if (tid == 0) thr = 1, cnt = 0;
+    __syncthreads();
+    uint32_t r = 0;
+#pragma unroll 8
+    for (uint32_t j = 0; j < 256; j++) r += best[j] > m;
+    if (m && r == k - 1) thr = m;
+    __syncthreads();
+    const u64 t = thr;
+    if (m >= t) {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const uint32_t i = (g + a.parts * e) * 1024 + 4 * tid;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const u64 w = word(l[e][j], i + j);
+                if (w >= t) list[atomicAdd(&cnt, 1u)] = w;
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t n = cnt;
+    u64 *const o = out + ((size_t)row * a.parts + g) * k;
+    for (uint32_t i = tid; i < n; i += 256) {
+        const u64 w = list[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; j++) rank += list[j] > w;
+        if (rank < k) o[rank] = w;
+    }
+    for (uint32_t i = n + tid; i < k; i += 256) o[i] = 0;
+}
+
+// The parts' words merged and the token picked.  The k-th largest of the first
+// ceil(k / parts) words of every part bounds the row's k-th from below; where
+// many words reach it (a few parts hold all the large ones), the k-th is found
+// by bisection instead of ranking each against each.
+__global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in) {
+    __shared__ __attribute__((aligned(16))) u64 list[PICK_MAX];
+    __shared__ __attribute__((aligned(16))) u64 head[MAX_PARTS + TK];
+    __shared__ u64 sel[TK], wt[TK];
+    __shared__ uint32_t at[TK], ok[TK];
+    __shared__ u64 thr;
+    __shared__ uint32_t cnt, nsel, tok;
+    const uint32_t tid = threadIdx.x, row = blockIdx.x, k = a.k, C = a.parts * k;
+    const uint32_t h = (k + a.parts - 1) / a.parts, H = a.parts * h;
+    in += (size_t)row * C;
+    for (uint32_t i = tid; i < H; i += 512) head[i] = in[(i / h) * k + i % h];
+    if (tid == 0) thr = 1, cnt = 0, nsel = 0, tok = 0xFFFFFFFFu;
+    __syncthreads();
+    for (uint32_t i = tid; i < H; i += 512) {
+        const u64 w = head[i];
+        uint32_t r = 0;
+        for (uint32_t j = 0; j < H; j++) r += head[j] > w;
+        if (w && r == k - 1) thr = w;
+    }
+    __syncthreads();
+    u64 t = thr;
+    for (uint32_t i = tid; i < C; i += 512) {
+        const u64 w = in[i];
+        if (w >= t) list[atomicAdd(&cnt, 1u)] = w;
+    }
+    __syncthreads();
+    uint32_t n = cnt;
+    if (n > 1024) {
+        // the largest value that at least k words reach, bit by bit
+        t = 0;
+        for (int b = 63; b >= 0; b--) {
+            const u64 c = t | 1ull << b;
+            uint32_t r = 0;
+            for (uint32_t i = tid; i < n; i += 512) r += list[i] >= c;
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) r += __shfl_xor(r, o, 64);
+            __syncthreads();
+            if (tid == 0) cnt = 0;
+            __syncthreads();
+            if ((tid & 63) == 0) atomicAdd(&cnt, r);
+            __syncthreads();
+            if (cnt >= k) t = c;
+        }
+        for (uint32_t i = tid; i < n; i += 512)
+            if (list[i] >= t) head[atomicAdd(&nsel, 1u)] = list[i];
+        __syncthreads();
+        n = nsel;
+        if (tid < n) list[tid] = head[tid];
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < n; i += 512) {
+        const u64 w = list[i];
+        uint32_t r = 0;
+        for (uint32_t j = 0; j < n; j++) r += list[j] > w;
+        if (r < k) sel[r] = w;
+    }
+    __syncthreads();
+    n = min(n, k);
+    if (n == 0) {
+        if (tid == 0) emit(a, row, 0xFFFFFFFFu, 0.f);
+        return;
+    }
+    const float top = word_logit(sel[0]);
+    double w = 0.0;
+    if (tid < n) {
+        w = weight(word_logit(sel[tid]), top, a.inv_t);
+        wt[tid] = fixed(w);
+        at[tid] = word_index(sel[tid]);
+    }
+    __syncthreads();
+    u64 before = 0, all = 0;
+    bool keep = false;
+    if (tid < n) {
+        for (uint32_t j = 0; j < n; j++) {
+            all += wt[j];
+            before += j < tid ? wt[j] : 0ull;
+        }
+        keep = tid == 0 || ((a.top_p >= 1.f || (double)before < (double)a.top_p * (double)all) && w >= (double)a.min_p);
+        ok[tid] = keep;
+    }
+    __syncthreads();
+    u64 upto = 0, sum = 0;
+    uint32_t last = 0;  // the kept word of the highest index that has a weight
+    if (tid < n) {
+        for (uint32_t j = 0; j < n; j++) {
+            if (!ok[j]) continue;
+            sum += wt[j];
+            upto += at[j] <= at[tid] ? wt[j] : 0ull;
+            if (wt[j]) last = max(last, at[j]);
+        }
+        if (keep && (double)upto > row_u(a, row) * (double)sum) atomicMin(&tok, at[tid]);
+    }
+    __syncthreads();
+    if (tid < n && keep) {
+        const uint32_t c = tok == 0xFFFFFFFFu ? last : tok;
+        if (at[tid] == c) emit(a, row, c, (float)((double)wt[tid] / (double)sum));
+    }
+}
+
+// ---- any top_k --------------------------------------------------------------
+// What a row's workspace holds besides the parts' ranges and sums.
+struct Hist {
+    u64 mass[NB];
+    uint32_t count[NB];
+};
+struct Cut {  // where the cuts fall (k_collect's first workgroup, for k_finish)
+    uint32_t b_lo, b_hi, bk;  // top-p's cut in b_lo..b_hi, top-k's in bk (NB: none); bins before b_lo are kept
+    uint32_t rank_k;          // words of bk that top-k keeps
+    u64 before_lo, before_k, total;
+};
+struct Work {
+    uint2 *range;      // [rows][parts] {largest, smallest} ord, 0: none
+    u64 *sum;          // [rows][parts]
+    Hist *hist;        // [rows]
+    Cut *cut;          // [rows]
+    u64 *list;         // [rows][LIST]
+    uint32_t *n_list;  // [rows]
+};
+
+__device__ __forceinline__ bool cuts(const Row &a) { return a.k || a.top_p < 1.f; }
+
+__global__ __launch_bounds__(256) void k_range(Row a, Work w) {
+    __shared__ uint32_t mx[4], mn[4];
+    const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
+    const float *const x = a.x + row * a.ld;
+    if (cuts(a)) {
+        for (uint32_t i = g * 256 + tid; i < NB; i += a.parts * 256) w.hist[row].mass[i] = 0, w.hist[row].count[i] = 0;
+        if (g == 0 && tid == 0) w.n_list[row] = 0;
+    }
+    uint32_t hi = 0, lo = 0xFFFFFFFFu;
+    const uint32_t end = min(a.vocab, (g + 1) * a.part);
+    for (uint32_t i = g * a.part + 4 * tid; i < end; i += 1024) {
+        float l[4];
+        load4(a, x, i, l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t k = ord(l[j]);
+            hi = max(hi, k);
+            if (k) lo = min(lo, k);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        hi = max(hi, (uint32_t)__shfl_xor(hi, o, 64));
+        lo = min(lo, (uint32_t)__shfl_xor(lo, o, 64));
+    }
+    if ((tid & 63) == 0) mx[tid >> 6] = hi, mn[tid >> 6] = lo;
+    __syncthreads();
+    if (tid == 0)
+        w.range[(size_t)row * a.parts + g] =
+            make_uint2(max(max(mx[0], mx[1]), max(mx[2], mx[3])), min(min(mn[0], mn[1]), min(mn[2], mn[3])));
+}
+
+// the row's largest logit and the bins' scale, the same in every workgroup
+struct Scale {
+    float top, inv;
+    bool any;
+};
+__device__ __forceinline__ Scale row_scale(const Row &a, const Work &w, uint32_t row, uint32_t (&sh)[2]) {
+    if (threadIdx.x == 0) sh[0] = 0, sh[1] = 0xFFFFFFFFu;
+    __syncthreads();
+    if (threadIdx.x < a.parts) {
+        const uint2 r = w.range[(size_t)row * a.parts + threadIdx.x];
+        atomicMax(&sh[0], r.x);
+        atomicMin(&sh[1], r.y);
+    }
+    __syncthreads();
+    Scale s;
+    s.any = sh[0] != 0;
+    s.top = unord(sh[0]);
+    // a word 30 T below the top weighs less than 2^-43: the bins end there
+    const float width = fminf(s.top - unord(sh[1]), 30.f * a.temp);
+    s.inv = width > 0.f ? (float)(NB - 1) / width : 0.f;
+    return s;
+}
+// monotone in l (each step rounds monotonically); NB: never taken
+__device__ __forceinline__ uint32_t bin_of(float l, const Scale &s) {
+    if (!(l > -INFINITY)) return NB;
+    return l == s.top ? 0u : (uint32_t)fminf((s.top - l) * s.inv, (float)(NB - 1));
+}
+
+__global__ __launch_bounds__(256) void k_hist(Row a, Work w) {
+    __shared__ u64 mass[NB];
+    __shared__ uint32_t count[NB], sh[2];
+    const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
+    const float *const x = a.x + row * a.ld;
+    for (uint32_t i = tid; i < NB; i += 256) mass[i] = 0, count[i] = 0;
+    const Scale s = row_scale(a, w, row, sh);
+    const uint32_t end = min(a.vocab, (g + 1) * a.part);
+    for (uint32_t i = g * a.part + 4 * tid; i < end; i += 1024) {
+        float l[4];
+        load4(a, x, i, l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t b = bin_of(l[j], s);
+            if (b == NB) continue;
+            const u64 f = fixed(weight(l[j], s.top, a.inv_t));
+            if (f) atomicAdd(&mass[b], f);
+            atomicAdd(&count[b], 1u);
+        }
+    }
+    __syncthreads();
+    Hist &h = w.hist[row];
+    for (uint32_t i = tid; i < NB; i += 256) {
+        if (mass[i]) atomicAdd(&h.mass[i], mass[i]);
+        if (count[i]) atomicAdd(&h.count[i], count[i]);
+    }
+}
+
+// the bins of the cuts from the row's histogram, by a workgroup of 256
+__device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[257], uint32_t (&cs)[4], Cut &sh) {
+    constexpr uint32_t PER = NB / 256;
+    const uint32_t tid = threadIdx.x;
+    u64 m[PER], tm = 0;
+    uint32_t c[PER], tc = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) {
+        m[i] = h.mass[tid * PER + i];
+        c[i] = h.count[tid * PER + i];
+        tm += m[i];
+        tc += c[i];
+    }
+    // exclusive sums of the threads' bins: within the wavefront, then over the four
+    u64 im = tm;
+    uint32_t ic = tc;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 vm = __shfl_up(im, o, 64);
+        const uint32_t vc = __shfl_up(ic, o, 64);
+        if ((tid & 63) >= (uint32_t)o) im += vm, ic += vc;
+    }
+    if ((tid & 63) == 63) ms[tid >> 6] = im, cs[tid >> 6] = ic;
+    if (tid == 0) sh.bk = NB, sh.rank_k = 0, sh.b_lo = NB, sh.b_hi = NB;
+    __syncthreads();
+    u64 total = 0, pm = im - tm;
+    uint32_t n = 0, pc = ic - tc;
+    for (uint32_t i = 0; i < 4; i++) {
+        if (i < tid >> 6) pm += ms[i], pc += cs[i];
+        total += ms[i];
+        n += cs[i];
+    }
+    if (tid == 0) sh.total = total, sh.before_k = total, sh.before_lo = 0;
+    __syncthreads();
+    // top-k's bin: the first that brings the count to k
+    u64 bm = pm, after_k = 0;
+    if (a.k && n > a.k) {
+        uint32_t bc = pc;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            if (bc < a.k && bc + c[i] >= a.k) {
+                sh.bk = tid * PER + i;
+                sh.rank_k = a.k - bc;
+                sh.before_k = bm;
+                ms[256] = bm + m[i];
+            }
+            bc += c[i];
+            bm += m[i];
+        }
+    } else if (tid == 0) {
+        ms[256] = total;
+    }
+    __syncthreads();
+    after_k = ms[256];
+    if (a.top_p < 1.f) {
+        // K's sum is between before_k and after_k: top-p's cut is in the bins
+        // that bring the sum to top_p times either
+        const double lo = (double)a.top_p * (double)sh.before_k, hi = (double)a.top_p * (double)after_k;
+        bm = pm;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            const u64 nx = bm + m[i];
+            const bool first = tid * PER + i == 0;
+            if (((double)bm < lo || first) && (double)nx >= lo) sh.b_lo = tid * PER + i, sh.before_lo = bm;
+            if (((double)bm < hi || first) && (double)nx >= hi) sh.b_hi = tid * PER + i;
+            bm = nx;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        // top-k's bin alone where there is no top-p, none where there is neither
+        if (a.top_p >= 1.f) sh.b_lo = sh.b_hi = sh.bk, sh.before_lo = sh.before_k;
+        sh.b_lo = min(sh.b_lo, sh.bk);
+        sh.b_hi = min(sh.b_hi, sh.bk);
+        if (sh.b_lo == sh.bk) sh.before_lo = sh.before_k;
+    }
+    __syncthreads();
+    return sh;
+}
+
+__device__ __forceinline__ bool in_cuts(uint32_t b, const Cut &c) { return b < NB && ((b >= c.b_lo && b <= c.b_hi) || b == c.bk); }
+
+__global__ __launch_bounds__(256) void k_collect(Row a, Work w) {
+    __shared__ u64 ms[257], put[LIST];
+    __shared__ uint32_t cs[4], sh[2], base, cnt;
+    __shared__ Cut cut;
+    __shared__ u64 part[4];
+    const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
+    const float *const x = a.x + row * a.ld;
+    const Scale s = row_scale(a, w, row, sh);
+    Cut c = {NB, NB, NB, 0, 0, 0, 0};
+    if (cuts(a)) {
+        c = find_cuts(a, w.hist[row], ms, cs, cut);
+        if (g == 0 && tid == 0) w.cut[row] = c;
+    }
+    if (tid == 0) cnt = 0;
+    __syncthreads();
+    u64 sum = 0;
+    const uint32_t end = min(a.vocab, (g + 1) * a.part);
+    for (uint32_t i = g * a.part + 4 * tid; i < end; i += 1024) {
+        float l[4];
+        load4(a, x, i, l);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const uint32_t b = i + j < end ? bin_of(l[j], s) : NB;
+            if (b < c.b_lo) {
+                const double v = weight(l[j], s.top, a.inv_t);
+                if (v >= (double)a.min_p || l[j] == s.top) sum += fixed(v);
+            } else if (in_cuts(b, c)) {
+                const uint32_t at = atomicAdd(&cnt, 1u);
+                if (at < LIST) put[at] = word(l[j], i + j);
+            }
+        }
+    }
+    // the part's words behind those of other parts; a row with more than LIST
+    // is counted in full and not read from the list
+    __syncthreads();
+    if (tid == 0 && cnt) base = atomicAdd(&w.n_list[row], cnt);
+    __syncthreads();
+    if (cnt)
+        for (uint32_t i = tid; i < min(cnt, LIST) && base + i < LIST; i += 256) w.list[(size_t)row * LIST + base + i] = put[i];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if ((tid & 63) == 0) part[tid >> 6] = sum;
+    __syncthreads();
+    if (tid == 0) w.sum[(size_t)row * a.parts + g] = part[0] + part[1] + part[2] + part[3];
+}
+
+// sum over the workgroup of 1024, in every thread
+template <typename T>
+__device__ __forceinline__ T wg_sum(T v, T (&sh)[16]) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    T r = 0;
+    for (int i = 0; i < 16; i++) r += sh[i];
+    return r;
+}
+
+// The cuts among the collected words, the kept words' sums by part, and the
+// token.  Where more words share the cuts' bins than the list holds (equal
+// logits by the thousand), the cuts are found bit by bit over the row itself.
+__global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
+    __shared__ __attribute__((aligned(16))) u64 list[LIST];
+    __shared__ __attribute__((aligned(16))) u64 wt[LIST];  // weight; 0 where outside top-p's bins
+    __shared__ uint16_t bin[LIST];
+    __shared__ u64 part[MAX_PARTS], red[16], thr_k, thr;
+    __shared__ uint32_t redc[16], sh[2], tok, last;
+    const uint32_t tid = threadIdx.x, row = blockIdx.x;
+    const float *const x = a.x + row * a.ld;
+    const Scale s = row_scale(a, w, row, sh);
+    if (!s.any) {
+        if (tid == 0) emit(a, row, 0xFFFFFFFFu, 0.f);
+        return;
+    }
+    const bool cut = cuts(a);
+    Cut c = {NB, NB, NB, 0, 0, 0, 0};
+    uint32_t n = 0;
+    if (cut) {
+        c = w.cut[row];
+        n = w.n_list[row];
+    }
+    if (tid < a.parts) part[tid] = w.sum[(size_t)row * a.parts + tid];
+    if (tid == 0) thr_k = 0, thr = ~0ull, tok = 0xFFFFFFFFu, last = 0;
+    __syncthreads();
+    auto mass = [&](u64 v) { return fixed(weight(word_logit(v), s.top, a.inv_t)); };
+    if (cut && n <= LIST) {
+        for (uint32_t i = tid; i < n; i += 1024) {
+            const u64 v = w.list[(size_t)row * LIST + i];
+            const uint32_t b = bin_of(word_logit(v), s);
+            list[i] = v;
+            bin[i] = (uint16_t)b;
+            wt[i] = b >= c.b_lo && b <= c.b_hi ? mass(v) : 0;
+        }
+        __syncthreads();
+        u64 sk = 0;
+        if (c.bk < NB) {
+            for (uint32_t i = tid; i < n; i += 1024) {
+                const u64 v = list[i];
+                if (bin[i] != c.bk) continue;
+                uint32_t r = 0;
+                for (uint32_t j = 0; j < n; j++) r += list[j] > v && bin[j] == c.bk;
+                if (r == c.rank_k - 1) thr_k = v;
+            }
+            __syncthreads();
+            for (uint32_t i = tid; i < n; i += 1024)
+                if (bin[i] == c.bk && list[i] >= thr_k) sk += mass(list[i]);
+            sk = wg_sum(sk, red);
+        }
+        sk += c.before_k;
+        const double want = (double)a.top_p * (double)sk;
+        for (uint32_t i = tid; i < n; i += 1024) {
+            const u64 v = list[i];
+            const uint32_t b = bin[i];
+            if (v < thr_k || b < c.b_lo || b > c.b_hi) continue;
+            u64 before = c.before_lo;
+            for (uint32_t j = 0; j < n; j++) before += list[j] > v ? wt[j] : 0ull;
+            if (a.top_p < 1.f && before && (double)before >= want) continue;
+            atomicMin(&thr, v);
+            const float l = word_logit(v);
+            if (l == s.top || weight(l, s.top, a.inv_t) >= (double)a.min_p)
+                atomicAdd(&part[word_index(v) / a.part], wt[i]);
+        }
+        __syncthreads();
+    } else if (cut) {
+        // f(v): bit by bit the largest value for which enough() of the words
+        // not below it in bins lo..hi still holds
+        auto count_at = [&](u64 v, uint32_t lo, uint32_t hi) {
+            uint32_t r = 0;
+            for (uint32_t i = tid; i < a.vocab; i += 1024) {
+                const u64 q = word(x[i], i);
+                const uint32_t b = bin_of(x[i], s);
+                r += q >= v && b >= lo && b <= hi;
+            }
+            return wg_sum(r, redc);
+        };
+        auto mass_at = [&](u64 v, uint32_t lo, uint32_t hi) {
+            u64 r = 0;
+            for (uint32_t i = tid; i < a.vocab; i += 1024) {
+                const u64 q = word(x[i], i);
+                const uint32_t b = bin_of(x[i], s);
+                if (q >= v && b >= lo && b <= hi) r += mass(q);
+            }
+            return wg_sum(r, red);
+        };
+        u64 tk = 0, sk = c.before_k;
+        if (c.bk < NB) {
+            for (int b = 63; b >= 0; b--)
+                if (count_at(tk | 1ull << b, c.bk, c.bk) >= c.rank_k) tk |= 1ull << b;
+            sk += mass_at(tk, c.bk, c.bk);
+        }
+        u64 tp = tk;
+        if (a.top_p < 1.f) {
+            const double want = (double)a.top_p * (double)sk;
+            tp = 0;
+            for (int b = 63; b >= 0; b--) {
+                const u64 r = c.before_lo + mass_at(max(tp | 1ull << b, tk), c.b_lo, c.b_hi);
+                if (r && (double)r >= want) tp |= 1ull << b;
+            }
+            tp = max(tp, tk);
+        }
+        __syncthreads();
+        if (tid == 0) thr = max(tp, 1ull);
+        if (tid < a.parts) part[tid] = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < a.vocab; i += 1024) {
+            const uint32_t b = bin_of(x[i], s);
+            if (b == NB || !(b < c.b_lo || (b <= c.b_hi && word(x[i], i) >= thr))) continue;
+            const double v = weight(x[i], s.top, a.inv_t);
+            const u64 f = fixed(v);
+            if (f && (v >= (double)a.min_p || x[i] == s.top)) atomicAdd(&part[i / a.part], f);
+        }
+        __syncthreads();
+    }
+    // the part that the token is in, then the token
+    u64 sum = 0, pre = 0;
+    uint32_t g = a.parts, end_g = 0;
+    u64 at_g = 0;
+    for (uint32_t i = 0; i < a.parts; i++) sum += part[i];
+    const double want = row_u(a, row) * (double)sum;
+    for (uint32_t i = 0; i < a.parts; i++) {
+        if (part[i]) end_g = i;
+        if (g == a.parts && (double)(pre + part[i]) > want) g = i, at_g = pre;
+        pre += part[i];
+    }
+    const bool past = g == a.parts;  // u >= 1: the last kept word
+    if (past) {
+        g = end_g;
+        at_g = sum - part[g];
+    }
+    const u64 t = thr;
+    const uint32_t first = g * a.part, end = min(a.vocab, first + a.part), per = (end - first + 1023) / 1024;
+    auto kept_mass = [&](uint32_t i) -> u64 {
+        const float l = x[i];
+        const uint32_t b = bin_of(l, s);
+        if (b == NB || !(b < c.b_lo || (b <= c.b_hi && word(l, i) >= t))) return 0;
+        const double v = weight(l, s.top, a.inv_t);
+        return v >= (double)a.min_p || l == s.top ? fixed(v) : 0ull;
+    };
+    u64 mine = 0;
+    const uint32_t i0 = first + min(tid * per, end - first), i1 = min(i0 + per, end);
+    for (uint32_t i = i0; i < i1; i++) mine += kept_mass(i);
+    u64 inc = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 v = __shfl_up(inc, o, 64);
+        if ((tid & 63) >= (uint32_t)o) inc += v;
+    }
+    __syncthreads();
+    if ((tid & 63) == 63) red[tid >> 6] = inc;
+    __syncthreads();
+    u64 run = at_g + inc - mine;
+    for (uint32_t i = 0; i < tid >> 6; i++) run += red[i];
+    if (mine && (past || (double)(run + mine) > want)) {
+        u64 r = run;
+        for (uint32_t i = i0; i < i1; i++) {
+            const u64 f = kept_mass(i);
+            r += f;
+            if (!f) continue;
+            if (past) {
+                atomicMax(&last, i);
+            } else if ((double)r > want) {
+                atomicMin(&tok, i);
+                break;
+            }
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        const uint32_t i = past ? last : tok;
+        emit(a, row, i, i < a.vocab ? (float)((double)kept_mass(i) / (double)sum) : 0.f);
+    }
+}
+
+// parts of a row for the first form: pieces of 1024 words, E to a workgroup
+uint32_t part_pieces(uint32_t vocab, uint32_t *e) {
+    const uint32_t pieces = (vocab + 1023) / 1024;
+    *e = pieces <= 64 ? 1 : pieces <= 128 ? 2 : pieces <= 256 ? 4 : 8;
+    return (pieces + *e - 1) / *e;
+}
+// ... and for the second: about four workgroups per CU over all rows, each at
+// least 1024 words; a multiple of 4 words each, so that rows stay aligned
+uint32_t range_parts(uint32_t vocab, uint32_t rows, uint32_t *part) {
+    const uint32_t pieces = (vocab + 1023) / 1024;
+    uint32_t g = (1024 + rows - 1) / rows;
+    g = g < 4 ? 4 : g > 64 ? 64 : g;
+    if (g > pieces) g = pieces;
+    *part = ((vocab + g - 1) / g + 3) / 4 * 4;
+    return (vocab + *part - 1) / *part;
+}
+
+struct Plan {
+    bool first;
+    uint32_t e, parts, part, k;
+};
+Plan plan(uint32_t rows, uint32_t vocab, const lrs_sampling &p) {
+    Plan r = {};
+    r.k = p.temperature == 0.f ? 1 : p.top_k >= vocab ? 0 : p.top_k;
+    r.parts = part_pieces(vocab, &r.e);
+    r.first = r.k && r.k <= TK && r.parts <= MAX_PARTS && r.parts * r.k <= PICK_MAX;
+    if (!r.first) r.parts = range_parts(vocab, rows, &r.part);
+    return r;
+}
+
+}  // namespace
+
+size_t sample_work_bytes(uint32_t rows, uint32_t vocab, const lrs_sampling &p) {
+    const Plan r = plan(rows, vocab, p);
+    if (r.first) return (size_t)rows * r.parts * r.k * 8;
+    return (size_t)rows * (r.parts * 16 + sizeof(Hist) + sizeof(Cut) + LIST * 8 + 8);
+}
+
+hipError_t launch_sample(const float *x, size_t ld, uint32_t rows, uint32_t vocab, const lrs_sampling &p, const float *u,
+                         uint32_t *tok, float *prob, void *work, hipStream_t s, uint32_t *step, uint32_t *gen,
+                         uint32_t gen_cap) {
+    const Plan r = plan(rows, vocab, p);
+    Row a = {};
+    a.x = x;
+    a.ld = ld;
+    a.vocab = vocab;
+    a.parts = r.parts;
+    a.part = r.part;
+    a.temp = p.temperature;
+    a.inv_t = p.temperature > 0.f ? 1.0 / (double)p.temperature : 0.0;
+    a.top_p = p.top_p;
+    a.min_p = p.min_p;
+    a.k = r.k;
+    a.u = u;
+    a.tok = tok;
+    a.prob = prob;
+    a.step = step;
+    a.gen = gen;
+    a.gen_cap = gen_cap;
+    a.vec = (uintptr_t)x % 16 == 0 && ld % 4 == 0;
+    if (r.first) {
+        u64 *const w = (u64 *)work;
+        const dim3 g(r.parts, rows);
+        switch (r.e) {
+        case 1: hipLaunchKernelGGL(k_part<1>, g, dim3(256), 0, s, a, w); break;
+        case 2: hipLaunchKernelGGL(k_part<2>, g, dim3(256), 0, s, a, w); break;
+        case 4: hipLaunchKernelGGL(k_part<4>, g, dim3(256), 0, s, a, w); break;
+        default: hipLaunchKernelGGL(k_part<8>, g, dim3(256), 0, s, a, w); break;
+        }
+        hipLaunchKernelGGL(k_pick, dim3(rows), dim3(512), 0, s, a, (const u64 *)w);
+        return hipGetLastError();
+    }
+    Work w;
+    w.hist = (Hist *)work;
+    w.cut = (Cut *)(w.hist + rows);
+    w.list = (u64 *)(w.cut + rows);
+    w.sum = w.list + (size_t)rows * LIST;
+    w.range = (uint2 *)(w.sum + (size_t)rows * r.parts);
+    w.n_list = (uint32_t *)(w.range + (size_t)rows * r.parts);
+    const dim3 g(r.parts, rows);
+    hipLaunchKernelGGL(k_range, g, dim3(256), 0, s, a, w);
+    if (a.k || a.top_p < 1.f) hipLaunchKernelGGL(k_hist, g, dim3(256), 0, s, a, w);
+    hipLaunchKernelGGL(k_collect, g, dim3(256), 0, s, a, w);
+    hipLaunchKernelGGL(k_finish, dim3(rows), dim3(1024), 0, s, a, w);
+    return hipGetLastError();
+}
+
+}  // namespace lrs

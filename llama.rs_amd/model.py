@@ -14,7 +14,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import Context, ModelError, Weight, check, lib, Q4_K, Q6_K
+from . import Context, LrsSampling, ModelError, Weight, check, lib, sampling, Q4_K, Q6_K
 
 _u32p = C.POINTER(C.c_uint32)
 _f32p = C.POINTER(C.c_float)
@@ -66,6 +66,12 @@ def _bind():
         "lrs_model_len": (C.c_uint32, [vp]),
         "lrs_decode_greedy": (C.c_int, [vp, C.c_uint32, C.c_uint32, _u32p]),
         "lrs_generate_greedy": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, vp]),
+        "lrs_decode_sample": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.POINTER(LrsSampling), C.c_float, _u32p]),
+        "lrs_generate_sample": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(LrsSampling), vp,
+                                          vp]),
+        "lrs_decode_tree": (C.c_int, [vp, vp, vp, C.c_uint32, C.c_uint32, vp]),
+        "lrs_tree_keep": (C.c_int, [vp, vp, C.c_uint32]),
+        "lrs_verify_tree": (C.c_int, [vp, vp, vp, C.c_uint32, C.c_uint32, C.POINTER(LrsSampling), vp, vp, _u32p]),
         "lrs_model_profile": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.POINTER(C.c_float),
                                         C.POINTER(C.c_size_t)]),
         "lrs_model_bytes_per_token": (C.c_size_t, [vp]),
@@ -81,6 +87,14 @@ _bind()
 
 CONFIG_KEYS = ("n_layer", "n_embd", "n_head", "n_head_kv", "head_dim", "n_ff", "vocab",
                "rope_dim", "ctx", "rms_eps", "freq_base")
+
+
+def _tree(tokens, parents):
+    t = np.ascontiguousarray(tokens, dtype=np.uint32).ravel()
+    p = np.ascontiguousarray(np.asarray(parents, np.int64) & 0xFFFFFFFF, dtype=np.uint32).ravel()
+    if t.size != p.size:
+        raise ModelError(-1, f"{t.size} tokens and {p.size} parents")
+    return t, p
 
 
 def _f32(a):
@@ -157,6 +171,56 @@ class ResidentForward:
         check(lib.lrs_generate_greedy(self.h, p.ctypes.data, p.size, int(pos0), int(n_gen),
                                       out.ctypes.data))
         return out
+
+    # --- device-side sampling (options: temperature, top_k, top_p, min_p) ----
+    def decode_sample(self, token: int, pos: int, u: float, **options) -> int:
+        """decode, then one token of its logits from the random number u in
+        [0, 1) (lrs_sample_dev's rule)."""
+        nxt = C.c_uint32()
+        check(lib.lrs_decode_sample(self.h, int(token), int(pos), C.byref(sampling(**options)), float(u),
+                                    C.byref(nxt)))
+        return int(nxt.value)
+
+    def generate_sample(self, prompt, u, pos0: int = 0, **options) -> np.ndarray:
+        """generate_greedy with token i sampled from u[i]."""
+        p = np.ascontiguousarray(prompt, dtype=np.uint32)
+        u = np.ascontiguousarray(u, dtype=np.float32)
+        out = np.empty(u.size, np.uint32)
+        check(lib.lrs_generate_sample(self.h, p.ctypes.data, p.size, int(pos0), u.size,
+                                      C.byref(sampling(**options)), u.ctypes.data, out.ctypes.data))
+        return out
+
+    # --- trees of drafted tokens (dense models) ------------------------------
+    def decode_tree(self, tokens, parents, pos0: int, logits: bool = True):
+        """The logits [n, vocab] of a tree of drafted tokens in one pass: node i
+        (parent parents[i] < i, -1: the last cached position) at position
+        pos0 + depth.  tree_keep takes a path of it into the cache."""
+        t, p = _tree(tokens, parents)
+        out = np.empty((t.size, self.vocab), np.float32) if logits else None
+        check(lib.lrs_decode_tree(self.h, t.ctypes.data, p.ctypes.data, t.size, int(pos0),
+                                  out.ctypes.data if logits else None))
+        return out
+
+    def tree_keep(self, nodes) -> None:
+        a = np.ascontiguousarray(nodes, dtype=np.uint32)
+        check(lib.lrs_tree_keep(self.h, a.ctypes.data, a.size))
+
+    def verify_tree(self, tokens, parents, pos0: int, u=None, **options) -> np.ndarray:
+        """One step of speculative decoding: node 0 is the last token, the others
+        its drafted continuations; returns the sampled tokens (u[i] for node i;
+        None: greedy), of which all but the last are in the cache then."""
+        t, p = _tree(tokens, parents)
+        if u is None:
+            options = dict(options, temperature=options.get("temperature", 0.0))
+        else:
+            u = np.ascontiguousarray(u, dtype=np.float32)
+            if u.size != t.size:
+                raise ModelError(-1, f"{u.size} random numbers for {t.size} nodes")
+        out, n = np.empty(max(t.size, 1), np.uint32), C.c_uint32()
+        check(lib.lrs_verify_tree(self.h, t.ctypes.data, p.ctypes.data, t.size, int(pos0),
+                                  C.byref(sampling(**options)), None if u is None else u.ctypes.data,
+                                  out.ctypes.data, C.byref(n)))
+        return out[:n.value].copy()
 
     OPS = {"qkv": 0, "attn": 1, "o": 2, "gateup": 3, "down": 4, "head": 5,
            "dn_proj": 6, "dn_step": 7, "dn_out": 8, "qk_prep": 9, "ffn": 10,
