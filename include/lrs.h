@@ -302,8 +302,7 @@ int lrs_tree_mask(const uint32_t *parents, uint32_t n, uint32_t *mask, uint32_t 
  * cache exact, q and p to 22 bits, f32 sums); a token that sees nothing has
  * zeros.  What a token does not see does not reach it, NaN and inf included.
  * q_dev, out_dev [n][n_head * head_dim], 16-byte aligned, not the same.  Async
- * on the context stream; uses at most 8 MB of the context scratch, its first
- * size. */
+ * on the context stream; uses up to 17 MB of the context scratch. */
 int lrs_attn_tree_dev(lrs_ctx *ctx, const lrs_kv *kv, const float *q_dev, uint32_t n, uint32_t n_head, uint32_t len,
                       const uint32_t *mask_dev, float scale, float *out_dev);
 

@@ -213,8 +213,9 @@ struct AttnTree {
     float *part;                   // [S][n][n_head * hd]
     float2 *ml;                    // [S][n][n_head]: {maximum (of powers of two), sum}
 };
-constexpr size_t TREE_WORK = 8u << 20;  // attn_tree_work_bytes is never above
-uint32_t attn_tree_splits(uint32_t n, uint32_t len, uint32_t n_head, uint32_t n_kv, uint32_t hd);
+// attn_tree_work_bytes is never above: shares are of at most 512 workgroups (256 at
+// head_dim 256) of 64 rows of head_dim floats and a float2
+constexpr size_t TREE_WORK = 17u << 20;
 size_t attn_tree_work_bytes(uint32_t n, uint32_t len, uint32_t n_head, uint32_t n_kv, uint32_t hd);
 hipError_t launch_attn_tree(AttnTree a, uint32_t hd, void *work, hipStream_t s);
 // out: {length, sampled tokens} of the walk from node 0, path: its nodes

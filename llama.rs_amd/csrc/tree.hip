@@ -7,6 +7,8 @@
 // 3584-4170) takes a chain of tokens.
 #include "gemm_pack.h"
 
+#include <algorithm>
+
 namespace lrs {
 
 // ---- rotation + append ------------------------------------------------------
@@ -123,18 +125,22 @@ hipError_t launch_rope_append(const RopeAppend &a, hipStream_t s) {
 
 // ---- attention --------------------------------------------------------------
 // Rows: the n nodes' queries of the KV head's group, row = node * rep + head in
-// the group, in tiles of 32.  A wavefront takes one tile and every NW-th chunk
-// of 32 positions of its workgroup's share; the workgroup's wavefronts are
-// merged through LDS, workgroups by k_tree_merge.  As in the prompt block's
-// kernel S^T = K Q^T and O^T = V^T P^T run on v_mfma_f32_32x32x16_f16 with the
-// exact f16 cache and q and p as f16 hi + lo (22 bits); here K and V come
-// straight from the cache into the operand registers, with no LDS and no
-// barrier in the loop: a lane holds 16 bytes of one position's K per K-step, and
-// HD / 32 neighbouring dims of each of its positions' V, which it repacks
-// two positions at a time; O^T tile t then holds dims HD / 32 * i + t.
+// the group, in tiles of 32.  A workgroup has T tiles and G groups of positions,
+// a wavefront for each pair: group p takes every G-th chunk of 32 positions of the
+// workgroup's share.  A chunk's K and V come to LDS with global_load_lds (the next
+// chunk's are in flight during the current one's products), where the group's T
+// wavefronts read them.  As in the prompt block's kernel S^T = K Q^T and
+// O^T = V^T P^T run on v_mfma_f32_32x32x16_f16 with the exact f16 cache and q and p
+// as f16 hi + lo (22 bits).  K's rows are XOR-swizzled (conflict-free 16-byte reads),
+// V comes from its rows by transposing reads (ds_read_b64_tr_b16).
+// The subtracted maximum follows the scores only when one exceeds it by 2^8: then
+// the sums are rescaled; p stays below 2^8, which f32 sums and f16 pairs hold.
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __fp16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef __fp16 h16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) h16x4_t lds_h16x4_t;
+typedef __attribute__((address_space(3))) void lds_void_t;
 
 // the 32 positions from 32 c on that row `node` sees
 __device__ __forceinline__ uint32_t seen_bits(const AttnTree &a, uint32_t node, uint32_t c) {
@@ -156,18 +162,38 @@ __device__ __forceinline__ uint32_t seen_bits(const AttnTree &a, uint32_t node, 
     return k >= 32 ? 0xFFFFFFFFu : ((1u << k) - 1) | word(0) << k;
 }
 
-template <int HD, int NW>
-__global__ __launch_bounds__(64 * NW) void k_attn_tree(AttnTree a) {
-    constexpr int KS = HD / 16;  // K-steps of S^T
-    constexpr int OT = HD / 32;  // tiles of O^T = dims of a lane's V
-    constexpr int LD = HD + 4;
-    __shared__ __attribute__((aligned(16))) float osum[32 * LD];
-    __shared__ float2 wml[NW][32];
+// the larger of the two half wavefronts' x, in both
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// wavefronts per SIMD that the LDS of as many workgroups as fit allows, at most 2
+// (the registers' limit at head_dim 128; 1 at 256)
+constexpr int tree_waves(int HD, int T, int G) {
+    const int lds = G * HD * 256 + G * T * 256;
+    return HD < 256 && 163840 / lds * T * G >= 8 ? 2 : 1;
+}
+
+template <int HD, int T, int G>
+__global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(AttnTree a) {
+    constexpr int KS = HD / 16;     // K-steps of S^T
+    constexpr int OT = HD / 32;     // tiles of O^T = dims of a lane's V
+    constexpr int NPR = HD / 8;     // 16-byte pieces of a row
+    constexpr int NI = HD / 16;     // 1 KB loads of a chunk's K or V
+    // A transposing read of 32 lanes takes 64 bytes of each of four rows: V's 16-byte
+    // pieces are turned by the row (row >> VT & VM, times 4) so that those are in
+    // different banks
+    constexpr uint32_t VT = HD == 64 ? 1 : 0, VM = HD == 64 ? 1 : 3;
+    // K, then V of a group's chunk of even and of odd rounds; the groups' sums at the end
+    __shared__ __attribute__((aligned(16))) _Float16 buf0[G][64 * HD], buf1[G][64 * HD];
+    __shared__ float2 wml[G][T * 32];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hf = lane >> 5, col = lane & 31;
-    const uint32_t rep = a.n_head / a.n_kv, rows = a.n * rep;
+    const uint32_t tw = wave % T, grp = wave / T;
+    const uint32_t rep = a.n_head / a.n_kv, rows = a.n * rep, tgs = (a.tiles + T - 1) / T;
     // the KV head goes fastest, so that with eight of them an XCD keeps one
-    // head's rows in its L2, then the tile, which shares them
-    const uint32_t g = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv % a.tiles, sp = blockIdx.x / a.n_kv / a.tiles;
+    // head's rows in its L2, then the tiles, which share them
+    const uint32_t g = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv % tgs * T + tw, sp = blockIdx.x / a.n_kv / tgs;
     const uint32_t r0 = 32 * tile + col, r = min(r0, rows - 1);  // lanes past the rows compute a copy
     const uint32_t node = r / rep, h = g * rep + r % rep;
     const uint32_t P = a.len + a.n, nch = (P - 1) / 32 + 1;
@@ -175,6 +201,27 @@ __global__ __launch_bounds__(64 * NW) void k_attn_tree(AttnTree a) {
     const _Float16 *const kb = a.kc + (size_t)g * a.rows * HD;
     const _Float16 *const vb = a.vc + (size_t)g * a.rows * HD;
 
+    uint32_t v_at[OT];
+    {
+        const uint32_t row = 4 * hf + (lane >> 2 & 3);
+#pragma unroll
+        for (int t = 0; t < OT; t++)
+            v_at[t] = row * HD + 8 * (4 * t ^ ((row >> VT & VM) << 2)) + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+    }
+    // chunk c -> the even or odd rounds' buffer: slot s (16 B) of K holds row s / NPR, piece
+    // (s % NPR) ^ (row % NPR).  Past the end: a row that is there.
+    auto stage = [&](uint32_t c, const bool odd) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t i = 0; i < (NI + T - 1) / T; i++) {
+            const uint32_t j = i * T + tw;
+            if (NI % T && j >= NI) break;
+            const uint32_t sl = 64 * j + lane, row = sl / NPR, pc = sl % NPR;
+            const size_t at = (size_t)min(32 * c + row, P - 1) * HD;
+            __builtin_amdgcn_global_load_lds(kb + at + 8 * (pc ^ (row % NPR)), (lds_void_t *)((odd ? buf1[grp] : buf0[grp]) + 512 * j), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(vb + at + 8 * (pc ^ ((row >> VT & VM) << 2)), (lds_void_t *)((odd ? buf1[grp] : buf0[grp]) + 32 * HD + 512 * j), 16, 0, 0);
+        }
+    };
+    const uint32_t first = c0 + grp;
     f16x8_t qh[KS], ql[KS];
     float qsc;
     {
@@ -186,19 +233,27 @@ __global__ __launch_bounds__(64 * NW) void k_attn_tree(AttnTree a) {
             const float4 v = *reinterpret_cast<const float4 *>(qp + 16 * k + 4);
             qv[k][0] = u.x, qv[k][1] = u.y, qv[k][2] = u.z, qv[k][3] = u.w;
             qv[k][4] = v.x, qv[k][5] = v.y, qv[k][6] = v.z, qv[k][7] = v.w;
+        }
+        // q's loads before the first chunk's: loads return in order
+        if (first < c1) stage(first, false);
+#pragma unroll
+        for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++) qm = fmaxf(qm, fabsf(qv[k][e]));
-        }
-        qm = fmaxf(qm, __shfl_xor(qm, 32, 64));
+        qm = half_max(qm);
         int ex;
         (void)frexpf(qm, &ex);
         ex = ex < -60 ? -60 : ex;
-        qsc = ldexpf(1.0f, ex) * a.scale * 1.4426950408889634f;  // scores in powers of two
+        // the scores' factor is positive (the maximum is taken before it): the
+        // scale's sign goes into q
+        const float sgn = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+        qsc = a.scale == 0.f ? 1.f : ldexpf(fabsf(a.scale) * 1.4426950408889634f, ex);  // in powers of two
+        const float down = ldexpf(sgn, -ex);
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float x = ldexpf(qv[k][e], -ex);
+                const float x = qv[k][e] * down;
                 const _Float16 xh = (_Float16)x;
                 qh[k][e] = xh;
                 ql[k][e] = (_Float16)(x - (float)xh);
@@ -209,250 +264,302 @@ __global__ __launch_bounds__(64 * NW) void k_attn_tree(AttnTree a) {
     for (int t = 0; t < OT; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[t][i] = 0.f;
-    float m = -INFINITY, l = 0.f;
-
-    f16x8_t kf[KS];
-    auto load_k = [&](uint32_t c) __attribute__((always_inline)) {
-        const uint32_t kp = min(32 * c + col, P - 1);  // past the end: a row that is there (not seen)
-        const _Float16 *const p = kb + (size_t)kp * HD + 8 * hf;
-#pragma unroll
-        for (int k = 0; k < KS; k++) kf[k] = *reinterpret_cast<const f16x8_t *>(p + 16 * k);
-    };
-    if (c0 + wave < c1) load_k(c0 + wave);
-    for (uint32_t c = c0 + wave; c < c1; c += NW) {
-        // V of position 16 s + 8 (j / 4) + 4 hf + j % 4: slot j of step s
-        uint32_t vr[2][8][OT / 2];
-#pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t kp = min(32 * c + 16 * s + 8 * (j >> 2) + 4 * hf + (j & 3), P - 1);
-                const uint32_t *const p = reinterpret_cast<const uint32_t *>(vb + (size_t)kp * HD) + OT / 2 * col;
-                if constexpr (OT == 8) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-                    vr[s][j][0] = v.x, vr[s][j][1] = v.y, vr[s][j][2] = v.z, vr[s][j][3] = v.w;
-                } else if constexpr (OT == 4) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-                    vr[s][j][0] = v.x, vr[s][j][1] = v.y;
-                } else {
-                    vr[s][j][0] = *p;
-                }
-            }
+    float m = -INFINITY, l = 0.f;  // l: of the lane's own positions
+    // the products of chunk c in buffer b; masked (a constant): it has positions that some
+    // rows do not see
+    auto chunk = [&](const bool masked, uint32_t c, const _Float16 *b) __attribute__((always_inline)) {
+        const _Float16 *const Kc = b, *const Vc = b + 32 * HD;
+        const uint32_t mine = masked ? seen_bits(a, node, c) >> (4 * hf) : 0xFFFFFFFFu;
         f32x16_t sc;
 #pragma unroll
         for (int i = 0; i < 16; i++) sc[i] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], ql[k], sc, 0, 0, 0);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qh[k], sc, 0, 0, 0);
+            const f16x8_t kf = *reinterpret_cast<const f16x8_t *>(Kc + 8 * (col * NPR + ((2 * k + hf) ^ (col % NPR))));
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], sc, 0, 0, 0);
         }
-        if (c + NW < c1) load_k(c + NW);
         // the lane's scores are positions 8 (i / 4) + 4 hf + i % 4
-        const bool masked = 32 * c + 32 > a.len;
-        uint32_t seen = 0xFFFFFFFFu;
-        if (masked) seen = seen_bits(a, node, c);
-        const uint32_t mine = seen >> (4 * hf);
-        float cmax = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float x = sc[i] * qsc;
-            sc[i] = mine >> (8 * (i >> 2) + (i & 3)) & 1 ? x : -INFINITY;
-            cmax = fmaxf(cmax, sc[i]);
-        }
-        cmax = fmaxf(cmax, __shfl_xor(cmax, 32, 64));
-        // a row that has seen nothing yet has only -inf: any finite maximum gives zeros
-        const float mn = fmaxf(m, cmax) == -INFINITY ? -1e30f : fmaxf(m, cmax);
-        const float alpha = __builtin_amdgcn_exp2f(m - mn);
-        float ps = 0.f;
-        f16x8_t ph[2], pl[2];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float p = __builtin_amdgcn_exp2f(sc[i] - mn);
-            ps += p;
-            const _Float16 x = (_Float16)p;
-            ph[i >> 3][i & 7] = x;
-            pl[i >> 3][i & 7] = (_Float16)(p - (float)x);
-        }
-        ps += __shfl_xor(ps, 32, 64);
-        l = l * alpha + ps;
-        m = mn;
-#pragma unroll
-        for (int t = 0; t < OT; t++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[t][i] *= alpha;
-        // a V that is not finite reaches the rows that see it alone: it is taken
-        // out of the product (0 inf is NaN) and added where it is seen
-        bool odd = false;
         if (masked) {
 #pragma unroll
-            for (int s = 0; s < 2; s++)
+            for (int i = 0; i < 16; i++) sc[i] = mine >> (8 * (i >> 2) + (i & 3)) & 1 ? sc[i] : -INFINITY;
+        }
+        float cmax = sc[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) cmax = fmaxf(cmax, sc[i]);
+        cmax = half_max(cmax) * qsc;
+        if (__any(cmax > m + 8.f)) {
+            const float mn = fmaxf(m, cmax);
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < OT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[t][i] *= alpha;
+        }
+        // a row that has seen nothing yet has only -inf: any finite maximum gives zeros
+        const float ms = m == -INFINITY ? 0.f : m;
+        f16x8_t ph[2], pl[2];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qsc, -ms));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i + 1], qsc, -ms));
+            l += p0;
+            l += p1;
+            const f16x2_t hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+            const f16x2_t lo = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi[0], -1.f, p0), __builtin_fmaf((float)hi[1], -1.f, p1));
+            ph[i >> 3][i & 7] = (_Float16)hi[0], ph[i >> 3][(i & 7) + 1] = (_Float16)hi[1];
+            pl[i >> 3][i & 7] = (_Float16)lo[0], pl[i >> 3][(i & 7) + 1] = (_Float16)lo[1];
+        }
+        // the transposing read gives lane i of sixteen column i of four rows, from
+        // addresses of four elements each: V of positions 16 s + 8 (j / 4) + 4 hf
+        // + j % 4, slots j of step s, for dim 32 t + lane % 32
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            f16x8_t va[OT];
+#pragma unroll
+            for (int t = 0; t < OT; t++) {
+                const _Float16 *const p = Vc + v_at[t] + 16 * s * HD;
+                const h16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h16x4_t *)p);
+                const h16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h16x4_t *)(p + 8 * HD));
+#pragma unroll
+                for (int j = 0; j < 4; j++) va[t][j] = (_Float16)lo[j], va[t][j + 4] = (_Float16)hi[j];
+            }
+            // a V that is not finite reaches the rows that see it alone: it is taken
+            // out of the product (0 inf is NaN) and added where it is seen
+            if (masked) {
+                f16x8_t one;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
+                    one[j] = mine >> (16 * s + 8 * (j >> 2) + (j & 3)) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
 #pragma unroll
-                    for (int w = 0; w < OT / 2; w++)
-                        odd |= (vr[s][j][w] & 0x7C00u) == 0x7C00u || (vr[s][j][w] & 0x7C000000u) == 0x7C000000u;
-            odd = __any(odd);
-        }
-        if (odd) {
-            f16x8_t one[2];
+                for (int t = 0; t < OT; t++) {
+                    bool odd = false;
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                one[i >> 3][i & 7] = mine >> (8 * (i >> 2) + (i & 3)) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
-            for (int t = 0; t < OT; t++) {
-                for (int kind = 0; kind < 3; kind++) {  // NaN, inf, -inf
-                    f32x16_t n;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) n[i] = 0.f;
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
+                    for (int j = 0; j < 8; j++) odd |= !(__builtin_fabsf16(va[t][j]) <= (_Float16)65504.0f);
+                    if (!__any(odd)) continue;
+#pragma unroll 1
+                    for (int kind = 0; kind < 3; kind++) {  // NaN, inf, -inf
                         f16x8_t is;
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
-                            uint32_t w = 0;
-#pragma unroll
-                            for (int i = 0; i < OT / 2; i++) w = i == t / 2 ? vr[s][j][i] : w;
-                            const uint32_t b = t & 1 ? w >> 16 : w & 0xFFFFu;
-                            const bool hit = kind == 0 ? (b & 0x7FFFu) > 0x7C00u : b == (kind == 1 ? 0x7C00u : 0xFC00u);
+                            const _Float16 v = va[t][j];
+                            const bool hit = kind == 0 ? v != v : v == (kind == 1 ? (_Float16)INFINITY : -(_Float16)INFINITY);
                             is[j] = hit ? (_Float16)1.0f : (_Float16)0.0f;
                         }
-                        n = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, one[s], n, 0, 0, 0);
-                    }
-                    const float val = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+                        f32x16_t n;
 #pragma unroll
-                    for (int q = 0; q < OT; q++)
+                        for (int i = 0; i < 16; i++) n[i] = 0.f;
+                        n = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, one, n, 0, 0, 0);
+                        const float val = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
 #pragma unroll
                         for (int i = 0; i < 16; i++)
-                            if (q == t && n[i] > 0.f) o[q][i] += val;
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int w = 0; w < OT / 2; w++) {
-                        if ((vr[s][j][w] & 0x7C00u) == 0x7C00u) vr[s][j][w] &= 0xFFFF0000u;
-                        if ((vr[s][j][w] & 0x7C000000u) == 0x7C000000u) vr[s][j][w] &= 0xFFFFu;
+                            if (n[i] > 0.f) o[t][i] += val;
                     }
-        }
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int t = 0; t < OT; t++) {
-                u32x4_t w;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    w[j] = __builtin_amdgcn_perm(vr[s][2 * j + 1][t / 2], vr[s][2 * j][t / 2], t & 1 ? 0x07060302u : 0x05040100u);
-                const f16x8_t va = __builtin_bit_cast(f16x8_t, w);
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[s], o[t], 0, 0, 0);
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[s], o[t], 0, 0, 0);
-            }
-    }
-    // the wavefronts' sums over the common maximum, one after another
-    if (hf == 0) wml[wave][col] = make_float2(m, l);
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; w++) M = fmaxf(M, wml[w][col].x);
-#pragma unroll
-    for (int w = 0; w < NW; w++) {
-        const float2 p = wml[w][col];
-        if (p.y != 0.f) L += p.y * __builtin_amdgcn_exp2f(p.x - M);
-    }
-    const float f = l != 0.f ? __builtin_amdgcn_exp2f(m - M) : 0.f;
-    for (int w = 0; w < NW; w++) {
-        if (wave == (uint32_t)w) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float *const p = osum + col * LD + OT * (8 * (i >> 2) + 4 * hf + (i & 3));
-#pragma unroll
-                for (int t = 0; t < OT; t++) {
-                    const float v = l != 0.f ? o[t][i] * f : 0.f;
-                    p[t] = w ? p[t] + v : v;
+                    for (int j = 0; j < 8; j++)
+                        if (!(__builtin_fabsf16(va[t][j]) <= (_Float16)65504.0f)) va[t][j] = (_Float16)0.0f;
                 }
             }
+            // neighbouring products go to different sums
+#pragma unroll
+            for (int t = 0; t < OT; t++) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[t], pl[s], o[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < OT; t++) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[t], ph[s], o[t], 0, 0, 0);
         }
+    };
+    // the same rounds for every group; the first `plain` of them are of positions
+    // that every row sees.  The two buffers are objects of their own and the
+    // plain rounds' parity is fixed, so that the compiler need not wait for the
+    // loads into one before it reads the other
+    const uint32_t rounds = c1 > c0 ? (c1 - c0 + G - 1) / G : 0, whole = min(c1, a.len / 32);
+    const uint32_t plain = whole > c0 ? (whole - c0) / G : 0;
+    auto next = [&](uint32_t it, const bool odd) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
+        if (first + (it + 1) * G < c1) stage(first + (it + 1) * G, !odd);
+    };
+    uint32_t it = 0;
+    for (; it + 1 < plain; it += 2) {
+        next(it, false);
+        chunk(false, first + it * G, buf0[grp]);
+        next(it + 1, true);
+        chunk(false, first + (it + 1) * G, buf1[grp]);
     }
-    // a tile's rows: heads of a node are neighbours in out and in the partials
-    if (a.S > 1 && wave == 0 && hf == 0 && r0 < rows) a.ml[((size_t)sp * a.n + node) * a.n_head + h] = make_float2(M, L);
-    if (wave == 0 && hf == 0) wml[0][col].x = L != 0.f ? 1.0f / L : 0.f;
+    for (; it < rounds; it++) {
+        next(it, it & 1);
+        if (first + it * G < c1) chunk(true, first + it * G, it & 1 ? buf1[grp] : buf0[grp]);
+    }
+    l += __shfl_xor(l, 32, 64);
+    float M = m, L = l, f = 1.f;
+    if constexpr (G > 1) {
+        // the groups' sums over the common maximum
+        if (hf == 0) wml[grp][tw * 32 + col] = make_float2(m, l);
+        __syncthreads();  // and every group has read its last chunk
+        M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < G; w++) M = fmaxf(M, wml[w][tw * 32 + col].x);
+#pragma unroll
+        for (int w = 0; w < G; w++) {
+            const float2 p = wml[w][tw * 32 + col];
+            if (p.y != 0.f) L += p.y * __builtin_amdgcn_exp2f(p.x - M);
+        }
+        f = l != 0.f ? __builtin_amdgcn_exp2f(m - M) : 0.f;
+    }
+    const size_t row_at = ((size_t)node * a.n_head + h) * HD;
+    if (grp == 0 && hf == 0 && a.S > 1 && r0 < rows) a.ml[((size_t)sp * a.n + node) * a.n_head + h] = make_float2(M, L);
+    f *= a.S > 1 ? 1.f : L != 0.f ? 1.f / L : 0.f;
+    float *const out = a.S > 1 ? a.part + (size_t)sp * a.n * a.n_head * HD : a.out;
+    // a lane's runs of four elements: at 32 t + 8 i + 4 hf
+    auto run = [&](int t, int i) {
+        return l != 0.f ? make_float4(o[t][4 * i] * f, o[t][4 * i + 1] * f, o[t][4 * i + 2] * f, o[t][4 * i + 3] * f)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    if constexpr (G == 1) {
+        if (r0 >= rows) return;
+#pragma unroll
+        for (int t = 0; t < OT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) *reinterpret_cast<float4 *>(out + row_at + 32 * t + 8 * i + 4 * hf) = run(t, i);
+        return;
+    }
+    // each group's tile t into its own buffer t (of 32 rows; the row's pieces of four
+    // elements turned by the row, so that the lanes of a write are in different banks)
+    static_assert(G == 1 || T <= 2, "a group has two buffers");
+    float *const mine = reinterpret_cast<float *>(tw ? buf1[grp] : buf0[grp]) + col * HD;
+#pragma unroll
+    for (int t = 0; t < OT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) *reinterpret_cast<float4 *>(mine + 4 * ((8 * t + 2 * i + hf) ^ (col % (HD / 4)))) = run(t, i);
     __syncthreads();
-    for (uint32_t i = tid; i < 32 * (HD / 4); i += 64 * NW) {
-        const uint32_t q = i / (HD / 4), d = 4 * (i % (HD / 4)), row = 32 * tile + q;
+    for (uint32_t i = tid; i < T * 32 * (HD / 4); i += 64 * T * G) {
+        const uint32_t q = i / (HD / 4), d = i % (HD / 4), row = 32 * (tile - tw) + q;
         if (row >= rows) break;
-        const float4 v = *reinterpret_cast<const float4 *>(osum + q * LD + d);
-        const size_t at = ((size_t)(row / rep) * a.n_head + g * rep + row % rep) * HD + d;
-        if (a.S > 1) {
-            *reinterpret_cast<float4 *>(a.part + (size_t)sp * a.n * a.n_head * HD + at) = v;
-        } else {
-            const float inv = wml[0][q].x;
-            *reinterpret_cast<float4 *>(a.out + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < G; w++) {
+            const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(q < 32 ? buf0[w] : buf1[w]) +
+                                                               (q % 32) * HD + 4 * (d ^ (q % (HD / 4))));
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        *reinterpret_cast<float4 *>(out + ((size_t)(row / rep) * a.n_head + g * rep + row % rep) * HD + 4 * d) = v;
+    }
+}
+
+// The workgroups' shares of a row joined: F threads (a power of two) for each 4
+// elements, which take every F-th share.  Load latency bounds it: a thread's shares
+// go by in fours.
+__global__ __launch_bounds__(256) void k_tree_merge(AttnTree a, uint32_t hd, uint32_t F) {
+    __shared__ float4 sv[256];
+    __shared__ float2 sm[256];
+    const uint32_t tid = threadIdx.x, e4 = hd / 4, per = e4 * F;
+    const uint32_t f = tid % per / e4, e = 4 * (tid % e4);
+    const size_t R = (size_t)a.n * a.n_head, r = (size_t)blockIdx.x * (256 / per) + tid / per, N = R * hd;
+    float M = -INFINITY, L = 0.f, v[4] = {};
+    if (r < R)
+        for (uint32_t s0 = f; s0 < a.S; s0 += 4 * F) {
+            float2 p[4];
+            float4 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t s = min(s0 + i * F, a.S - 1);
+                p[i] = a.ml[s * R + r];
+                x[i] = *reinterpret_cast<const float4 *>(a.part + s * N + r * hd + e);
+                if (s0 + i * F >= a.S) p[i] = make_float2(-INFINITY, 0.f);
+            }
+            const float mn = fmaxf(M, fmaxf(fmaxf(p[0].x, p[1].x), fmaxf(p[2].x, p[3].x)));
+            const float al = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+            L *= al;
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] *= al;
+            M = mn;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (p[i].y == 0.f) continue;  // saw nothing
+                const float w = __builtin_amdgcn_exp2f(p[i].x - M);
+                L = fmaf(p[i].y, w, L);
+                v[0] = fmaf(w, x[i].x, v[0]), v[1] = fmaf(w, x[i].y, v[1]);
+                v[2] = fmaf(w, x[i].z, v[2]), v[3] = fmaf(w, x[i].w, v[3]);
+            }
+        }
+    if (F > 1) {
+        sv[tid] = make_float4(v[0], v[1], v[2], v[3]);
+        sm[tid] = make_float2(M, L);
+        __syncthreads();
+        if (f) return;
+        float mn = M;
+        for (uint32_t i = 1; i < F; i++) mn = fmaxf(mn, sm[tid + i * e4].x);
+        const float al = L != 0.f ? __builtin_amdgcn_exp2f(M - mn) : 0.f;
+        L *= al;
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = L != 0.f ? v[k] * al : 0.f;
+        for (uint32_t i = 1; i < F; i++) {
+            const float2 p = sm[tid + i * e4];
+            const float4 x = sv[tid + i * e4];
+            if (p.y == 0.f) continue;
+            const float w = __builtin_amdgcn_exp2f(p.x - mn);
+            L = fmaf(p.y, w, L);
+            v[0] = fmaf(w, x.x, v[0]), v[1] = fmaf(w, x.y, v[1]), v[2] = fmaf(w, x.z, v[2]), v[3] = fmaf(w, x.w, v[3]);
         }
     }
-}
-
-// the workgroups' shares of a row joined: thread = 4 elements of a row
-__global__ __launch_bounds__(256) void k_tree_merge(AttnTree a, uint32_t hd) {
-    const size_t e = 4 * ((size_t)blockIdx.x * 256 + threadIdx.x), N = (size_t)a.n * a.n_head * hd;
-    if (e >= N) return;
-    const size_t r = e / hd;
-    float M = -INFINITY;
-    for (uint32_t s = 0; s < a.S; s++) M = fmaxf(M, a.ml[(size_t)s * a.n * a.n_head + r].x);
-    float L = 0.f, v[4] = {};
-#pragma unroll 4
-    for (uint32_t s = 0; s < a.S; s++) {
-        const float2 p = a.ml[(size_t)s * a.n * a.n_head + r];
-        const float4 x = *reinterpret_cast<const float4 *>(a.part + (size_t)s * N + e);
-        if (p.y == 0.f) continue;  // saw nothing
-        const float w = __builtin_amdgcn_exp2f(p.x - M);
-        L = fmaf(p.y, w, L);
-        v[0] = fmaf(w, x.x, v[0]), v[1] = fmaf(w, x.y, v[1]), v[2] = fmaf(w, x.z, v[2]), v[3] = fmaf(w, x.w, v[3]);
-    }
+    if (r >= R) return;
     const float inv = L != 0.f ? 1.0f / L : 0.f;
-    *reinterpret_cast<float4 *>(a.out + e) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    *reinterpret_cast<float4 *>(a.out + r * hd + e) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
 }
 
-static constexpr uint32_t TREE_NW = 4;
-
-// shares of the positions: about two workgroups per CU, each wavefront at least
-// a chunk, and no more partial sums than TREE_WORK holds
-uint32_t attn_tree_splits(uint32_t n, uint32_t len, uint32_t n_head, uint32_t n_kv, uint32_t hd) {
-    const uint32_t tiles = (n * (n_head / n_kv) + 31) / 32, wgs = tiles * n_kv, chunks = (len + n - 1) / 32 + 1;
-    const size_t fit = TREE_WORK / ((size_t)n * n_head * (hd * 4 + 8));
-    uint32_t S = (512 + wgs - 1) / wgs;
-    S = S < (chunks + TREE_NW - 1) / TREE_NW ? S : (chunks + TREE_NW - 1) / TREE_NW;
-    if (S > fit) S = fit ? (uint32_t)fit : 1;
+// Tiles and position groups of a workgroup, and shares of the positions: four
+// wavefronts a workgroup (two at head_dim 256, whose buffers are twice as large),
+// of two tiles where there are two; a workgroup per CU, and two (the second
+// wavefront of a SIMD, whose products overlap the first's softmax) where a
+// wavefront then still has eight chunks: 64 nodes of the 32B shape behind 130000
+// positions 413 -> 369 us, 26 behind 3900 22 -> 26 us.
+struct TreeShape {
+    uint32_t T, G, S;
+};
+static TreeShape tree_shape(uint32_t n, uint32_t len, uint32_t n_head, uint32_t n_kv, uint32_t hd) {
+    const uint32_t tiles = (n * (n_head / n_kv) + 31) / 32, chunks = (len + n - 1) / 32 + 1;
+    TreeShape r;
+    r.T = tiles == 1 ? 1 : 2;
+    r.G = hd == 256 ? 2 / r.T : 4 / r.T;
+    const uint32_t wgs = (tiles + r.T - 1) / r.T * n_kv;
+    const uint32_t full = hd < 256 && (uint64_t)chunks * wgs >= 512u * 8 * r.G ? 512 : 256;
+    const uint32_t S = std::max(1u, std::min(full / wgs, (chunks + r.G - 1) / r.G));
     // no empty share
     const uint32_t share = (chunks + S - 1) / S;
-    return (chunks + share - 1) / share;
+    r.S = (chunks + share - 1) / share;
+    return r;
 }
 
 size_t attn_tree_work_bytes(uint32_t n, uint32_t len, uint32_t n_head, uint32_t n_kv, uint32_t hd) {
-    const uint32_t S = attn_tree_splits(n, len, n_head, n_kv, hd);
+    const uint32_t S = tree_shape(n, len, n_head, n_kv, hd).S;
     return S > 1 ? (size_t)S * n * n_head * (hd * 4 + 8) : 0;
 }
 
 hipError_t launch_attn_tree(AttnTree a, uint32_t hd, void *work, hipStream_t s) {
-    const uint32_t rep = a.n_kv ? a.n_head / a.n_kv : 0;
-    if (a.n == 0 || rep == 0 || a.n_head % a.n_kv) return hipErrorInvalidValue;
-    a.tiles = (a.n * rep + 31) / 32;
-    a.S = attn_tree_splits(a.n, a.len, a.n_head, a.n_kv, hd);
+    if (a.n == 0 || a.n_kv == 0 || a.n_head == 0 || a.n_head % a.n_kv) return hipErrorInvalidValue;
+    const TreeShape sh = tree_shape(a.n, a.len, a.n_head, a.n_kv, hd);
+    a.tiles = (a.n * (a.n_head / a.n_kv) + 31) / 32;
+    a.S = sh.S;
     if (a.S > 1) {
         if (!work) return hipErrorInvalidValue;
         a.part = (float *)work;
         a.ml = (float2 *)(a.part + (size_t)a.S * a.n * a.n_head * hd);
     }
-    const dim3 g(a.n_kv * a.tiles * a.S), b(64 * TREE_NW);
-    switch (hd) {
-    case 64: hipLaunchKernelGGL((k_attn_tree<64, TREE_NW>), g, b, 0, s, a); break;
-    case 128: hipLaunchKernelGGL((k_attn_tree<128, TREE_NW>), g, b, 0, s, a); break;
-    case 256: hipLaunchKernelGGL((k_attn_tree<256, TREE_NW>), g, b, 0, s, a); break;
-    default: return hipErrorInvalidValue;
-    }
+    void (*fn)(AttnTree) = nullptr;
+#define LRS_TREE(H, T_, G_) \
+    if (hd == H && sh.T == T_ && sh.G == G_) fn = k_attn_tree<H, T_, G_>;
+    LRS_TREE(64, 1, 4) LRS_TREE(64, 2, 2)
+    LRS_TREE(128, 1, 4) LRS_TREE(128, 2, 2)
+    LRS_TREE(256, 1, 2) LRS_TREE(256, 2, 1)
+#undef LRS_TREE
+    if (!fn) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(fn, dim3((a.tiles + sh.T - 1) / sh.T * a.n_kv * a.S), dim3(64 * sh.T * sh.G), 0, s, a);
     if (a.S > 1) {
-        const size_t q = (size_t)a.n * a.n_head * hd / 4;
-        hipLaunchKernelGGL(k_tree_merge, dim3((uint32_t)((q + 255) / 256)), dim3(256), 0, s, a, hd);
+        uint32_t F = 1;
+        while (F < 1024 / hd && 4 * F < a.S) F *= 2;
+        const uint32_t rows = 256 / (hd / 4 * F);
+        hipLaunchKernelGGL(k_tree_merge, dim3((a.n * a.n_head + rows - 1) / rows), dim3(256), 0, s, a, hd, F);
     }
     return hipGetLastError();
 }
