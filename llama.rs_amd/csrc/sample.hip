@@ -37,7 +37,7 @@ constexpr uint32_t TK = 128;        // top_k of the first form
 constexpr uint32_t PICK_MAX = 8192; // words that a row's parts give it at most
 constexpr uint32_t NB = 2048;       // bins of the second form
 constexpr uint32_t LIST = 2048;     // words of the cuts' bins kept per row
-constexpr uint32_t MAX_PARTS = 256;
+constexpr uint32_t MAX_PARTS = 256;  // of the first form; 64 of the second, one for each lane
 constexpr double ONE = 4398046511104.0;  // 2^42
 
 struct Row {
@@ -52,7 +52,8 @@ struct Row {
     float *prob;           // or null
     uint32_t *step, *gen;  // the token as the next step's too (row 0), or null
     uint32_t gen_cap;
-    bool vec;  // rows are 16-byte aligned
+    bool vec;     // rows are 16-byte aligned
+    bool listed;  // second form: every word that top-k may keep is in the row's list
 };
 
 // the logit as an unsigned number of the same order; 0: never taken
@@ -72,11 +73,34 @@ __device__ __forceinline__ u64 word(float l, uint32_t i) {
 __device__ __forceinline__ uint32_t word_index(u64 w) { return 0xFFFFFFFFu - (uint32_t)w; }
 __device__ __forceinline__ float word_logit(u64 w) { return unord((uint32_t)(w >> 32)); }
 
+// e^x, x <= 0 (0 below -800): e^x = 2^n e^r with |r| <= ln 2 / 2, the series to
+// r^11 (r^12 / 12! < 2^-47 of it)
+__device__ __forceinline__ double exp_neg(double x) {
+    x = fmax(x, -800.0);
+    const double n = rint(x * 1.4426950408889634);
+    const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, x));
+    double p = 1.0 / 39916800;
+    p = fma(p, r, 1.0 / 3628800);
+    p = fma(p, r, 1.0 / 362880);
+    p = fma(p, r, 1.0 / 40320);
+    p = fma(p, r, 1.0 / 5040);
+    p = fma(p, r, 1.0 / 720);
+    p = fma(p, r, 1.0 / 120);
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
 // e^((l - top) / T), 1 for the top's equals (an infinite top leaves the rest nothing)
 __device__ __forceinline__ double weight(float l, float top, double inv_t) {
-    return l == top ? 1.0 : exp(((double)l - (double)top) * inv_t);
+    return l == top ? 1.0 : exp_neg(((double)l - (double)top) * inv_t);
 }
-__device__ __forceinline__ u64 fixed(double w) { return (u64)(w * ONE + 0.5); }
+// in whole multiples of 2^-42: the sum with 2^52 rounds to one
+__device__ __forceinline__ u64 fixed(double w) {
+    return (u64)__double_as_longlong(w * ONE + 4503599627370496.0) - 0x4330000000000000ull;
+}
 
 // l[0..4) of elements i.. of a row, -inf past its end
 __device__ __forceinline__ void load4(const Row &a, const float *x, uint32_t i, float (&l)[4]) {
@@ -89,9 +113,11 @@ __device__ __forceinline__ void load4(const Row &a, const float *x, uint32_t i, 
     }
 }
 
-__device__ __forceinline__ double row_u(const Row &a, uint32_t row) {
+// the token is the first word at which the running sum (of whole numbers) is
+// above this: floor(u sum), below sum itself
+__device__ __forceinline__ u64 target(const Row &a, uint32_t row, u64 sum) {
     const float u = a.u[row];
-    return u > 0.f ? (double)u : 0.0;
+    return u > 0.f ? (u < 1.f ? min((u64)((double)u * (double)sum), sum - 1) : sum - 1) : 0ull;
 }
 
 __device__ __forceinline__ void emit(const Row &a, uint32_t row, uint32_t tok, float p) {
@@ -107,92 +133,140 @@ __device__ __forceinline__ void emit(const Row &a, uint32_t row, uint32_t tok, f
 }
 
 // ---- top_k up to TK -------------------------------------------------------
-// The top_k words of a part (pieces g, g + parts, .. of 1024 words), descending,
-// zeros behind them.  The k-th largest of the 256 threads' own maxima bounds
-// them from below, so that of a part's words little more than k are ranked
-// against one another, at most k threads' all.
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// how many of list's words (zeros behind them up to a multiple of 8) are above w;
+// the reads of eight words are in flight together
+__device__ __forceinline__ uint32_t above(const u64 *list, uint32_t n, u64 w) {
+    uint32_t r = 0;
+    for (uint32_t j = 0; j < n; j += 8) {
+        u64x2 v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = *reinterpret_cast<const u64x2 *>(list + j + 2 * e);
+#pragma unroll
+        for (int e = 0; e < 4; e++) r += (v[e][0] > w) + (v[e][1] > w);
+    }
+    return r;
+}
+
+// The top_k words of a part (pieces g, g + parts, .. of 1024 words): word j of
+// part g in out[j][g], descending, zeros behind them.  The k-th largest of the 256
+// threads' own maxima bounds them from below, so that of a part's words little more
+// than k are ranked against one another.  The bound is of the logits alone (a
+// compare of 64 bits takes four times one of 32); where equal logits bring more
+// words to it than the list holds, of whole words: then at most k threads' all.
 template <int E>
 __global__ __launch_bounds__(256) void k_part(Row a, u64 *__restrict__ out) {
-    __shared__ __attribute__((aligned(16))) u64 best[256];
-    __shared__ __attribute__((aligned(16))) u64 list[4 * E * TK];
+    __shared__ __attribute__((aligned(16))) uint32_t best[256];
+    __shared__ __attribute__((aligned(16))) u64 bestw[256];
+    __shared__ __attribute__((aligned(16))) u64 list[4 * E * TK + 8];
     __shared__ u64 thr;
-    __shared__ uint32_t cnt;
+    __shared__ uint32_t cnt, low;
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y, k = a.k;
     const float *const x = a.x + row * a.ld;
     float l[E][4];
-    u64 m = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
         const size_t i = ((size_t)g + (size_t)a.parts * e) * 1024 + 4 * tid;
         load4(a, x, (uint32_t)min(i, (size_t)a.vocab), l[e]);
     }
+    if (tid == 0) low = 0xFFFFFFFFu, cnt = 0, thr = 1;
+    uint32_t m = 0;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const uint32_t i = (g + a.parts * e) * 1024 + 4 * tid;
+    for (int e = 0; e < E; e++)
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) m = max(m, word(l[e][j], i + j));
-    }
+        for (uint32_t j = 0; j < 4; j++) m = max(m, ord(l[e][j]));
     best[tid] = m;
-    if (tid == 0) thr = 1, cnt = 0;
     __syncthreads();
     uint32_t r = 0;
-#pragma unroll 8
-    for (uint32_t j = 0; j < 256; j++) r += best[j] > m;
-    if (m && r == k - 1) thr = m;
+#pragma unroll
+    for (uint32_t j = 0; j < 256; j += 32) {
+        u32x4 v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = *reinterpret_cast<const u32x4 *>(best + j + 4 * e);
+#pragma unroll
+        for (int e = 0; e < 8; e++) r += (v[e][0] > m) + (v[e][1] > m) + (v[e][2] > m) + (v[e][3] > m);
+    }
+    // the least of the maxima that fewer than k exceed; 0 where there are fewer than k
+    if (r < k) atomicMin(&low, m);
     __syncthreads();
-    const u64 t = thr;
-    if (m >= t) {
+    const uint32_t lo = max(low, 1u);
+    auto collect = [&](auto takes) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const uint32_t i = (g + a.parts * e) * 1024 + 4 * tid;
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
                 const u64 w = word(l[e][j], i + j);
-                if (w >= t) list[atomicAdd(&cnt, 1u)] = w;
+                if (takes(w)) {
+                    const uint32_t at = atomicAdd(&cnt, 1u);
+                    if (at < 4 * E * TK) list[at] = w;
+                }
             }
         }
-    }
+    };
+    if (m >= lo) collect([&](u64 w) { return (uint32_t)(w >> 32) >= lo; });
     __syncthreads();
+    if (cnt > 4 * E * TK) {
+        u64 mw = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) mw = max(mw, word(l[e][j], (g + a.parts * e) * 1024 + 4 * tid + j));
+        bestw[tid] = mw;
+        __syncthreads();
+        if (tid == 0) cnt = 0;
+        if (mw && above(bestw, 256, mw) == k - 1) thr = mw;
+        __syncthreads();
+        const u64 t = thr;
+        collect([&](u64 w) { return w >= t; });
+        __syncthreads();
+    }
     const uint32_t n = cnt;
-    u64 *const o = out + ((size_t)row * a.parts + g) * k;
+    if (tid < 8) list[n + tid] = 0;
+    __syncthreads();
+    u64 *const o = out + (size_t)row * a.parts * k + g;
     for (uint32_t i = tid; i < n; i += 256) {
         const u64 w = list[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; j++) rank += list[j] > w;
-        if (rank < k) o[rank] = w;
+        const uint32_t rank = above(list, n, w);
+        if (rank < k) o[(size_t)rank * a.parts] = w;
     }
-    for (uint32_t i = n + tid; i < k; i += 256) o[i] = 0;
+    for (uint32_t i = n + tid; i < k; i += 256) o[(size_t)i * a.parts] = 0;
 }
 
 // The parts' words merged and the token picked.  The k-th largest of the first
 // ceil(k / parts) words of every part bounds the row's k-th from below; where
 // many words reach it (a few parts hold all the large ones), the k-th is found
-// by bisection instead of ranking each against each.
+// by bisection instead of ranking each against each.  One wavefront then picks,
+// two words a lane.
 __global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in) {
-    __shared__ __attribute__((aligned(16))) u64 list[PICK_MAX];
-    __shared__ __attribute__((aligned(16))) u64 head[MAX_PARTS + TK];
-    __shared__ u64 sel[TK], wt[TK];
-    __shared__ uint32_t at[TK], ok[TK];
+    struct Kept {
+        u64 w;
+        uint32_t at, pad;
+    };
+    __shared__ __attribute__((aligned(16))) u64 list[PICK_MAX + 8];
+    __shared__ __attribute__((aligned(16))) u64 head[MAX_PARTS + TK + 8];
+    __shared__ __attribute__((aligned(16))) u64 sel[TK];
+    __shared__ __attribute__((aligned(16))) Kept kept[TK + 4];
     __shared__ u64 thr;
-    __shared__ uint32_t cnt, nsel, tok;
+    __shared__ uint32_t cnt, nsel;
     const uint32_t tid = threadIdx.x, row = blockIdx.x, k = a.k, C = a.parts * k;
-    const uint32_t h = (k + a.parts - 1) / a.parts, H = a.parts * h;
+    const uint32_t H = a.parts * ((k + a.parts - 1) / a.parts);
     in += (size_t)row * C;
-    for (uint32_t i = tid; i < H; i += 512) head[i] = in[(i / h) * k + i % h];
-    if (tid == 0) thr = 1, cnt = 0, nsel = 0, tok = 0xFFFFFFFFu;
+    u64 v[PICK_MAX / 512];
+#pragma unroll
+    for (uint32_t e = 0; e < PICK_MAX / 512; e++) v[e] = tid + 512 * e < C ? in[tid + 512 * e] : 0ull;
+    if (tid < H + 8) head[tid] = tid < H ? v[0] : 0ull;
+    if (tid < TK) sel[tid] = 0;
+    if (tid == 0) thr = 1, cnt = 0, nsel = 0;
     __syncthreads();
-    for (uint32_t i = tid; i < H; i += 512) {
-        const u64 w = head[i];
-        uint32_t r = 0;
-        for (uint32_t j = 0; j < H; j++) r += head[j] > w;
-        if (w && r == k - 1) thr = w;
-    }
+    if (tid < H && v[0] && above(head, H, v[0]) == k - 1) thr = v[0];
     __syncthreads();
     u64 t = thr;
-    for (uint32_t i = tid; i < C; i += 512) {
-        const u64 w = in[i];
-        if (w >= t) list[atomicAdd(&cnt, 1u)] = w;
-    }
+#pragma unroll
+    for (uint32_t e = 0; e < PICK_MAX / 512; e++)
+        if (v[e] >= t) list[atomicAdd(&cnt, 1u)] = v[e];
     __syncthreads();
     uint32_t n = cnt;
     if (n > 1024) {
@@ -218,53 +292,71 @@ __global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in)
         if (tid < n) list[tid] = head[tid];
         __syncthreads();
     }
+    if (tid < 8) list[n + tid] = 0;
+    __syncthreads();
     for (uint32_t i = tid; i < n; i += 512) {
         const u64 w = list[i];
-        uint32_t r = 0;
-        for (uint32_t j = 0; j < n; j++) r += list[j] > w;
+        const uint32_t r = above(list, n, w);
         if (r < k) sel[r] = w;
     }
     __syncthreads();
+    if (tid >= 64) return;
     n = min(n, k);
     if (n == 0) {
         if (tid == 0) emit(a, row, 0xFFFFFFFFu, 0.f);
         return;
     }
+    // lane i: words 2 i and 2 i + 1 of the order
     const float top = word_logit(sel[0]);
-    double w = 0.0;
-    if (tid < n) {
-        w = weight(word_logit(sel[tid]), top, a.inv_t);
-        wt[tid] = fixed(w);
-        at[tid] = word_index(sel[tid]);
+    u64 f[2], w[2];
+    double p[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        w[e] = sel[2 * tid + e];
+        p[e] = w[e] ? weight(word_logit(w[e]), top, a.inv_t) : 0.0;
+        f[e] = fixed(p[e]);
     }
-    __syncthreads();
-    u64 before = 0, all = 0;
-    bool keep = false;
-    if (tid < n) {
-        for (uint32_t j = 0; j < n; j++) {
-            all += wt[j];
-            before += j < tid ? wt[j] : 0ull;
+    u64 inc = f[0] + f[1];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 x = __shfl_up(inc, o, 64);
+        if (tid >= (uint32_t)o) inc += x;
+    }
+    const double want = (double)a.top_p * (double)__shfl(inc, 63, 64);
+    u64 before = inc - f[0] - f[1], sum = 0;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const bool keep = w[e] && ((tid == 0 && e == 0) || ((a.top_p >= 1.f || (double)before < want) && p[e] >= (double)a.min_p));
+        before += f[e];
+        if (!keep) f[e] = 0;
+        sum += f[e];
+        kept[2 * tid + e] = Kept{f[e], word_index(w[e]), 0};
+    }
+    if (tid < 4) kept[TK + tid] = Kept{0, 0, 0};
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    // a word's sum in index order, over the kept words
+    u64 upto[2] = {0, 0};
+    const uint32_t i0 = word_index(w[0]), i1 = word_index(w[1]);
+    for (uint32_t j = 0; j < n; j += 4) {
+        Kept q[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[e] = kept[j + e];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            upto[0] += q[e].at <= i0 ? q[e].w : 0ull;
+            upto[1] += q[e].at <= i1 ? q[e].w : 0ull;
         }
-        keep = tid == 0 || ((a.top_p >= 1.f || (double)before < (double)a.top_p * (double)all) && w >= (double)a.min_p);
-        ok[tid] = keep;
     }
-    __syncthreads();
-    u64 upto = 0, sum = 0;
-    uint32_t last = 0;  // the kept word of the highest index that has a weight
-    if (tid < n) {
-        for (uint32_t j = 0; j < n; j++) {
-            if (!ok[j]) continue;
-            sum += wt[j];
-            upto += at[j] <= at[tid] ? wt[j] : 0ull;
-            if (wt[j]) last = max(last, at[j]);
-        }
-        if (keep && (double)upto > row_u(a, row) * (double)sum) atomicMin(&tok, at[tid]);
-    }
-    __syncthreads();
-    if (tid < n && keep) {
-        const uint32_t c = tok == 0xFFFFFFFFu ? last : tok;
-        if (at[tid] == c) emit(a, row, c, (float)((double)wt[tid] / (double)sum));
-    }
+    const u64 past = target(a, row, sum);
+    uint32_t c = 0xFFFFFFFFu;
+    if (f[0] && upto[0] > past) c = i0;
+    if (f[1] && upto[1] > past) c = min(c, i1);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) c = min(c, (uint32_t)__shfl_xor(c, o, 64));
+    if (f[0] && i0 == c) emit(a, row, c, (float)(p[0] * ONE / (double)sum));
+    if (f[1] && i1 == c) emit(a, row, c, (float)(p[1] * ONE / (double)sum));
 }
 
 // ---- any top_k --------------------------------------------------------------
@@ -274,9 +366,11 @@ struct Hist {
     uint32_t count[NB];
 };
 struct Cut {  // where the cuts fall (k_collect's first workgroup, for k_finish)
-    uint32_t b_lo, b_hi, bk;  // top-p's cut in b_lo..b_hi, top-k's in bk (NB: none); bins before b_lo are kept
-    uint32_t rank_k;          // words of bk that top-k keeps
-    u64 before_lo, before_k, total;
+    // the bins of the list: top-p's cut is in b_lo..b_hi, top-k's in bk (NB: none);
+    // words of bins before b_lo are kept
+    uint32_t b_lo, b_hi, bk;
+    uint32_t rank_k;  // words of bk that top-k keeps
+    u64 before_lo, before_k;
 };
 struct Work {
     uint2 *range;      // [rows][parts] {largest, smallest} ord, 0: none
@@ -289,26 +383,35 @@ struct Work {
 
 __device__ __forceinline__ bool cuts(const Row &a) { return a.k || a.top_p < 1.f; }
 
+// f(logit, index) for the words of part g, by a workgroup of 256, sixteen words a
+// thread in flight
+template <typename F>
+__device__ __forceinline__ void for_words(const Row &a, const float *x, uint32_t g, F f) {
+    const uint32_t end = min(a.vocab, (g + 1) * a.part);
+    for (uint32_t i0 = g * a.part + 4 * threadIdx.x; i0 < end; i0 += 4096) {
+        float l[4][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) load4(a, x, i0 + 1024 * e < end ? i0 + 1024 * e : a.vocab, l[e]);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) f(l[e][j], i0 + 1024 * e + j);
+    }
+}
+
 __global__ __launch_bounds__(256) void k_range(Row a, Work w) {
     __shared__ uint32_t mx[4], mn[4];
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
-    const float *const x = a.x + row * a.ld;
     if (cuts(a)) {
         for (uint32_t i = g * 256 + tid; i < NB; i += a.parts * 256) w.hist[row].mass[i] = 0, w.hist[row].count[i] = 0;
         if (g == 0 && tid == 0) w.n_list[row] = 0;
     }
     uint32_t hi = 0, lo = 0xFFFFFFFFu;
-    const uint32_t end = min(a.vocab, (g + 1) * a.part);
-    for (uint32_t i = g * a.part + 4 * tid; i < end; i += 1024) {
-        float l[4];
-        load4(a, x, i, l);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t k = ord(l[j]);
-            hi = max(hi, k);
-            if (k) lo = min(lo, k);
-        }
-    }
+    for_words(a, a.x + row * a.ld, g, [&](float l, uint32_t) {
+        const uint32_t k = ord(l);
+        hi = max(hi, k);
+        lo = min(lo, k - 1);  // 0, never taken, is the largest
+    });
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
         hi = max(hi, (uint32_t)__shfl_xor(hi, o, 64));
@@ -318,28 +421,29 @@ __global__ __launch_bounds__(256) void k_range(Row a, Work w) {
     __syncthreads();
     if (tid == 0)
         w.range[(size_t)row * a.parts + g] =
-            make_uint2(max(max(mx[0], mx[1]), max(mx[2], mx[3])), min(min(mn[0], mn[1]), min(mn[2], mn[3])));
+            make_uint2(max(max(mx[0], mx[1]), max(mx[2], mx[3])), min(min(mn[0], mn[1]), min(mn[2], mn[3])) + 1);
 }
 
-// the row's largest logit and the bins' scale, the same in every workgroup
+// the row's largest logit and the bins' scale, the same in every wavefront
 struct Scale {
     float top, inv;
     bool any;
 };
-__device__ __forceinline__ Scale row_scale(const Row &a, const Work &w, uint32_t row, uint32_t (&sh)[2]) {
-    if (threadIdx.x == 0) sh[0] = 0, sh[1] = 0xFFFFFFFFu;
-    __syncthreads();
-    if (threadIdx.x < a.parts) {
-        const uint2 r = w.range[(size_t)row * a.parts + threadIdx.x];
-        atomicMax(&sh[0], r.x);
-        atomicMin(&sh[1], r.y);
+__device__ __forceinline__ Scale row_scale(const Row &a, const Work &w, uint32_t row) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint2 r = make_uint2(0u, 0u);
+    if (lane < a.parts) r = w.range[(size_t)row * a.parts + lane];
+    r.y -= 1;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        r.x = max(r.x, (uint32_t)__shfl_xor(r.x, o, 64));
+        r.y = min(r.y, (uint32_t)__shfl_xor(r.y, o, 64));
     }
-    __syncthreads();
     Scale s;
-    s.any = sh[0] != 0;
-    s.top = unord(sh[0]);
+    s.any = r.x != 0;
+    s.top = unord(r.x);
     // a word 30 T below the top weighs less than 2^-43: the bins end there
-    const float width = fminf(s.top - unord(sh[1]), 30.f * a.temp);
+    const float width = fminf(s.top - unord(r.y + 1), 30.f * a.temp);
     s.inv = width > 0.f ? (float)(NB - 1) / width : 0.f;
     return s;
 }
@@ -349,47 +453,50 @@ __device__ __forceinline__ uint32_t bin_of(float l, const Scale &s) {
     return l == s.top ? 0u : (uint32_t)fminf((s.top - l) * s.inv, (float)(NB - 1));
 }
 
+// MASS: weights by bin too (not where the list will hold every word that counts)
+template <bool MASS>
 __global__ __launch_bounds__(256) void k_hist(Row a, Work w) {
-    __shared__ u64 mass[NB];
-    __shared__ uint32_t count[NB], sh[2];
+    __shared__ u64 mass[MASS ? NB : 1];
+    __shared__ uint32_t count[NB];
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
-    const float *const x = a.x + row * a.ld;
-    for (uint32_t i = tid; i < NB; i += 256) mass[i] = 0, count[i] = 0;
-    const Scale s = row_scale(a, w, row, sh);
-    const uint32_t end = min(a.vocab, (g + 1) * a.part);
-    for (uint32_t i = g * a.part + 4 * tid; i < end; i += 1024) {
-        float l[4];
-        load4(a, x, i, l);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t b = bin_of(l[j], s);
-            if (b == NB) continue;
-            const u64 f = fixed(weight(l[j], s.top, a.inv_t));
-            if (f) atomicAdd(&mass[b], f);
-            atomicAdd(&count[b], 1u);
-        }
+    const bool counts = a.k != 0;
+    for (uint32_t i = tid; i < NB; i += 256) {
+        if constexpr (MASS) mass[i] = 0;
+        count[i] = 0;
     }
+    const Scale s = row_scale(a, w, row);
+    __syncthreads();
+    for_words(a, a.x + row * a.ld, g, [&](float l, uint32_t) {
+        const uint32_t b = bin_of(l, s);
+        if (b == NB) return;
+        if constexpr (MASS) {
+            const u64 f = fixed(weight(l, s.top, a.inv_t));
+            if (f) atomicAdd(&mass[b], f);
+        }
+        if (counts) atomicAdd(&count[b], 1u);
+    });
     __syncthreads();
     Hist &h = w.hist[row];
     for (uint32_t i = tid; i < NB; i += 256) {
-        if (mass[i]) atomicAdd(&h.mass[i], mass[i]);
+        if constexpr (MASS)
+            if (mass[i]) atomicAdd(&h.mass[i], mass[i]);
         if (count[i]) atomicAdd(&h.count[i], count[i]);
     }
 }
 
 // the bins of the cuts from the row's histogram, by a workgroup of 256
-__device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[257], uint32_t (&cs)[4], Cut &sh) {
+__device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[5], uint32_t (&cs)[4], Cut &sh) {
     constexpr uint32_t PER = NB / 256;
     const uint32_t tid = threadIdx.x;
     u64 m[PER], tm = 0;
     uint32_t c[PER], tc = 0;
 #pragma unroll
     for (uint32_t i = 0; i < PER; i++) {
-        m[i] = h.mass[tid * PER + i];
+        m[i] = a.listed ? 0ull : h.mass[tid * PER + i];
         c[i] = h.count[tid * PER + i];
-        tm += m[i];
-        tc += c[i];
     }
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) tm += m[i], tc += c[i];
     // exclusive sums of the threads' bins: within the wavefront, then over the four
     u64 im = tm;
     uint32_t ic = tc;
@@ -400,7 +507,6 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
         if ((tid & 63) >= (uint32_t)o) im += vm, ic += vc;
     }
     if ((tid & 63) == 63) ms[tid >> 6] = im, cs[tid >> 6] = ic;
-    if (tid == 0) sh.bk = NB, sh.rank_k = 0, sh.b_lo = NB, sh.b_hi = NB;
     __syncthreads();
     u64 total = 0, pm = im - tm;
     uint32_t n = 0, pc = ic - tc;
@@ -409,11 +515,15 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
         total += ms[i];
         n += cs[i];
     }
-    if (tid == 0) sh.total = total, sh.before_k = total, sh.before_lo = 0;
-    __syncthreads();
     // top-k's bin: the first that brings the count to k
-    u64 bm = pm, after_k = 0;
-    if (a.k && n > a.k) {
+    const bool cut_k = a.k && n > a.k;
+    if (tid == 0) {
+        sh.b_lo = sh.b_hi = NB;
+        sh.before_lo = 0;
+        if (!cut_k) sh.bk = NB, sh.rank_k = 0, sh.before_k = ms[4] = total;
+    }
+    u64 bm = pm;
+    if (cut_k) {
         uint32_t bc = pc;
 #pragma unroll
         for (uint32_t i = 0; i < PER; i++) {
@@ -421,20 +531,19 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
                 sh.bk = tid * PER + i;
                 sh.rank_k = a.k - bc;
                 sh.before_k = bm;
-                ms[256] = bm + m[i];
+                ms[4] = bm + m[i];
             }
             bc += c[i];
             bm += m[i];
         }
-    } else if (tid == 0) {
-        ms[256] = total;
     }
     __syncthreads();
-    after_k = ms[256];
-    if (a.top_p < 1.f) {
-        // K's sum is between before_k and after_k: top-p's cut is in the bins
-        // that bring the sum to top_p times either
-        const double lo = (double)a.top_p * (double)sh.before_k, hi = (double)a.top_p * (double)after_k;
+    if (a.listed) {
+        if (tid == 0) sh.b_lo = 0, sh.b_hi = sh.bk, sh.before_k = 0;
+    } else if (a.top_p < 1.f) {
+        // K's sum is between its sums before and after top-k's bin: top-p's cut is in
+        // the bins that bring the sum to top_p times either
+        const double lo = (double)a.top_p * (double)sh.before_k, hi = (double)a.top_p * (double)ms[4];
         bm = pm;
 #pragma unroll
         for (uint32_t i = 0; i < PER; i++) {
@@ -446,12 +555,10 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
         }
     }
     __syncthreads();
-    if (tid == 0) {
-        // top-k's bin alone where there is no top-p, none where there is neither
-        if (a.top_p >= 1.f) sh.b_lo = sh.b_hi = sh.bk, sh.before_lo = sh.before_k;
+    if (tid == 0 && !a.listed) {
         sh.b_lo = min(sh.b_lo, sh.bk);
         sh.b_hi = min(sh.b_hi, sh.bk);
-        if (sh.b_lo == sh.bk) sh.before_lo = sh.before_k;
+        if (sh.b_lo == sh.bk) sh.before_lo = sh.before_k;  // top-k's bin alone where there is no top-p
     }
     __syncthreads();
     return sh;
@@ -460,37 +567,30 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
 __device__ __forceinline__ bool in_cuts(uint32_t b, const Cut &c) { return b < NB && ((b >= c.b_lo && b <= c.b_hi) || b == c.bk); }
 
 __global__ __launch_bounds__(256) void k_collect(Row a, Work w) {
-    __shared__ u64 ms[257], put[LIST];
-    __shared__ uint32_t cs[4], sh[2], base, cnt;
+    __shared__ u64 ms[5], put[LIST];
+    __shared__ uint32_t cs[4], base, cnt;
     __shared__ Cut cut;
     __shared__ u64 part[4];
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
-    const float *const x = a.x + row * a.ld;
-    const Scale s = row_scale(a, w, row, sh);
-    Cut c = {NB, NB, NB, 0, 0, 0, 0};
+    const Scale s = row_scale(a, w, row);
+    Cut c = {NB, NB, NB, 0, 0, 0};
+    if (tid == 0) cnt = 0;
     if (cuts(a)) {
         c = find_cuts(a, w.hist[row], ms, cs, cut);
         if (g == 0 && tid == 0) w.cut[row] = c;
     }
-    if (tid == 0) cnt = 0;
     __syncthreads();
     u64 sum = 0;
-    const uint32_t end = min(a.vocab, (g + 1) * a.part);
-    for (uint32_t i = g * a.part + 4 * tid; i < end; i += 1024) {
-        float l[4];
-        load4(a, x, i, l);
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            const uint32_t b = i + j < end ? bin_of(l[j], s) : NB;
-            if (b < c.b_lo) {
-                const double v = weight(l[j], s.top, a.inv_t);
-                if (v >= (double)a.min_p || l[j] == s.top) sum += fixed(v);
-            } else if (in_cuts(b, c)) {
-                const uint32_t at = atomicAdd(&cnt, 1u);
-                if (at < LIST) put[at] = word(l[j], i + j);
-            }
+    for_words(a, a.x + row * a.ld, g, [&](float l, uint32_t i) {
+        const uint32_t b = bin_of(l, s);
+        if (b < c.b_lo) {
+            const double v = weight(l, s.top, a.inv_t);
+            if (v >= (double)a.min_p || l == s.top) sum += fixed(v);
+        } else if (in_cuts(b, c)) {
+            const uint32_t at = atomicAdd(&cnt, 1u);
+            if (at < LIST) put[at] = word(l, i);
         }
-    }
+    });
     // the part's words behind those of other parts; a row with more than LIST
     // is counted in full and not read from the list
     __syncthreads();
@@ -514,6 +614,7 @@ __device__ __forceinline__ T wg_sum(T v, T (&sh)[16]) {
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     T r = 0;
+#pragma unroll
     for (int i = 0; i < 16; i++) r += sh[i];
     return r;
 }
@@ -522,61 +623,72 @@ __device__ __forceinline__ T wg_sum(T v, T (&sh)[16]) {
 // token.  Where more words share the cuts' bins than the list holds (equal
 // logits by the thousand), the cuts are found bit by bit over the row itself.
 __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
-    __shared__ __attribute__((aligned(16))) u64 list[LIST];
-    __shared__ __attribute__((aligned(16))) u64 wt[LIST];  // weight; 0 where outside top-p's bins
-    __shared__ uint16_t bin[LIST];
-    __shared__ u64 part[MAX_PARTS], red[16], thr_k, thr;
-    __shared__ uint32_t redc[16], sh[2], tok, last;
-    const uint32_t tid = threadIdx.x, row = blockIdx.x;
+    __shared__ __attribute__((aligned(16))) u64 list[LIST + 8];
+    __shared__ __attribute__((aligned(16))) u64 wt[LIST + 8];  // weight; 0 where outside top-p's bins
+    __shared__ u64 part[64], red[16], thr_k, thr;
+    __shared__ uint32_t redc[16];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
     const float *const x = a.x + row * a.ld;
-    const Scale s = row_scale(a, w, row, sh);
-    if (!s.any) {
-        if (tid == 0) emit(a, row, 0xFFFFFFFFu, 0.f);
-        return;
-    }
     const bool cut = cuts(a);
-    Cut c = {NB, NB, NB, 0, 0, 0, 0};
+    // the list's first words are read before its length is known
+    const u64 early = cut ? w.list[(size_t)row * LIST + tid] : 0ull;
+    Cut c = {NB, NB, NB, 0, 0, 0};
     uint32_t n = 0;
     if (cut) {
         c = w.cut[row];
         n = w.n_list[row];
     }
-    if (tid < a.parts) part[tid] = w.sum[(size_t)row * a.parts + tid];
-    if (tid == 0) thr_k = 0, thr = ~0ull, tok = 0xFFFFFFFFu, last = 0;
-    __syncthreads();
+    const Scale s = row_scale(a, w, row);
+    if (!s.any) {
+        if (tid == 0) emit(a, row, 0xFFFFFFFFu, 0.f);
+        return;
+    }
+    if (tid < 64) part[tid] = tid < a.parts ? w.sum[(size_t)row * a.parts + tid] : 0ull;
+    if (tid == 0) thr_k = 0, thr = ~0ull;
     auto mass = [&](u64 v) { return fixed(weight(word_logit(v), s.top, a.inv_t)); };
     if (cut && n <= LIST) {
+        uint32_t in_bk = 0;
         for (uint32_t i = tid; i < n; i += 1024) {
-            const u64 v = w.list[(size_t)row * LIST + i];
+            const u64 v = i < 1024 ? early : w.list[(size_t)row * LIST + i];
             const uint32_t b = bin_of(word_logit(v), s);
             list[i] = v;
-            bin[i] = (uint16_t)b;
             wt[i] = b >= c.b_lo && b <= c.b_hi ? mass(v) : 0;
+            in_bk += b == c.bk;
+        }
+        if (tid < 8) list[n + tid] = 0, wt[n + tid] = 0;
+        u64 sk = c.before_k;
+        if (c.bk < NB) {
+            // the list's other words are of earlier bins, above bk's
+            const uint32_t last = n - wg_sum(in_bk, redc) + c.rank_k - 1;
+            for (uint32_t i = tid; i < n; i += 1024)
+                if (above(list, n, list[i]) == last) thr_k = list[i];
         }
         __syncthreads();
-        u64 sk = 0;
-        if (c.bk < NB) {
-            for (uint32_t i = tid; i < n; i += 1024) {
-                const u64 v = list[i];
-                if (bin[i] != c.bk) continue;
-                uint32_t r = 0;
-                for (uint32_t j = 0; j < n; j++) r += list[j] > v && bin[j] == c.bk;
-                if (r == c.rank_k - 1) thr_k = v;
-            }
-            __syncthreads();
+        if (c.bk < NB || a.listed) {
+            u64 m = 0;
             for (uint32_t i = tid; i < n; i += 1024)
-                if (bin[i] == c.bk && list[i] >= thr_k) sk += mass(list[i]);
-            sk = wg_sum(sk, red);
+                if (list[i] >= thr_k && (a.listed || bin_of(word_logit(list[i]), s) == c.bk)) m += mass(list[i]);
+            sk += wg_sum(m, red);
         }
-        sk += c.before_k;
         const double want = (double)a.top_p * (double)sk;
         for (uint32_t i = tid; i < n; i += 1024) {
             const u64 v = list[i];
-            const uint32_t b = bin[i];
+            const uint32_t b = bin_of(word_logit(v), s);
             if (v < thr_k || b < c.b_lo || b > c.b_hi) continue;
-            u64 before = c.before_lo;
-            for (uint32_t j = 0; j < n; j++) before += list[j] > v ? wt[j] : 0ull;
-            if (a.top_p < 1.f && before && (double)before >= want) continue;
+            if (a.top_p < 1.f) {
+                u64 before = c.before_lo;
+                for (uint32_t j = 0; j < n; j += 4) {
+                    u64x2 q[2], f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        q[e] = *reinterpret_cast<const u64x2 *>(list + j + 2 * e);
+                        f[e] = *reinterpret_cast<const u64x2 *>(wt + j + 2 * e);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) before += (q[e][0] > v ? f[e][0] : 0ull) + (q[e][1] > v ? f[e][1] : 0ull);
+                }
+                if (before && (double)before >= want) continue;
+            }
             atomicMin(&thr, v);
             const float l = word_logit(v);
             if (l == s.top || weight(l, s.top, a.inv_t) >= (double)a.min_p)
@@ -584,8 +696,7 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
         }
         __syncthreads();
     } else if (cut) {
-        // f(v): bit by bit the largest value for which enough() of the words
-        // not below it in bins lo..hi still holds
+        // bit by bit the largest value that enough of the bins' words reach
         auto count_at = [&](u64 v, uint32_t lo, uint32_t hi) {
             uint32_t r = 0;
             for (uint32_t i = tid; i < a.vocab; i += 1024) {
@@ -605,11 +716,10 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
             return wg_sum(r, red);
         };
         u64 tk = 0, sk = c.before_k;
-        if (c.bk < NB) {
+        if (c.bk < NB)
             for (int b = 63; b >= 0; b--)
                 if (count_at(tk | 1ull << b, c.bk, c.bk) >= c.rank_k) tk |= 1ull << b;
-            sk += mass_at(tk, c.bk, c.bk);
-        }
+        if (c.bk < NB || a.listed) sk += mass_at(tk, a.listed ? 0 : c.bk, min(c.bk, NB - 1));
         u64 tp = tk;
         if (a.top_p < 1.f) {
             const double want = (double)a.top_p * (double)sk;
@@ -622,7 +732,7 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
         }
         __syncthreads();
         if (tid == 0) thr = max(tp, 1ull);
-        if (tid < a.parts) part[tid] = 0;
+        if (tid < 64) part[tid] = 0;
         __syncthreads();
         for (uint32_t i = tid; i < a.vocab; i += 1024) {
             const uint32_t b = bin_of(x[i], s);
@@ -632,64 +742,65 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
             if (f && (v >= (double)a.min_p || x[i] == s.top)) atomicAdd(&part[i / a.part], f);
         }
         __syncthreads();
+    } else {
+        __syncthreads();
     }
-    // the part that the token is in, then the token
-    u64 sum = 0, pre = 0;
-    uint32_t g = a.parts, end_g = 0;
-    u64 at_g = 0;
-    for (uint32_t i = 0; i < a.parts; i++) sum += part[i];
-    const double want = row_u(a, row) * (double)sum;
-    for (uint32_t i = 0; i < a.parts; i++) {
-        if (part[i]) end_g = i;
-        if (g == a.parts && (double)(pre + part[i]) > want) g = i, at_g = pre;
-        pre += part[i];
-    }
-    const bool past = g == a.parts;  // u >= 1: the last kept word
-    if (past) {
-        g = end_g;
-        at_g = sum - part[g];
-    }
-    const u64 t = thr;
-    const uint32_t first = g * a.part, end = min(a.vocab, first + a.part), per = (end - first + 1023) / 1024;
-    auto kept_mass = [&](uint32_t i) -> u64 {
-        const float l = x[i];
-        const uint32_t b = bin_of(l, s);
-        if (b == NB || !(b < c.b_lo || (b <= c.b_hi && word(l, i) >= t))) return 0;
-        const double v = weight(l, s.top, a.inv_t);
-        return v >= (double)a.min_p || l == s.top ? fixed(v) : 0ull;
-    };
-    u64 mine = 0;
-    const uint32_t i0 = first + min(tid * per, end - first), i1 = min(i0 + per, end);
-    for (uint32_t i = i0; i < i1; i++) mine += kept_mass(i);
+    // the part that the token is in: every wavefront adds up the parts, one a lane
+    const u64 mine = part[lane];
     u64 inc = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const u64 v = __shfl_up(inc, o, 64);
-        if ((tid & 63) >= (uint32_t)o) inc += v;
+        if (lane >= (uint32_t)o) inc += v;
     }
-    __syncthreads();
-    if ((tid & 63) == 63) red[tid >> 6] = inc;
-    __syncthreads();
-    u64 run = at_g + inc - mine;
-    for (uint32_t i = 0; i < tid >> 6; i++) run += red[i];
-    if (mine && (past || (double)(run + mine) > want)) {
-        u64 r = run;
-        for (uint32_t i = i0; i < i1; i++) {
-            const u64 f = kept_mass(i);
-            r += f;
-            if (!f) continue;
-            if (past) {
-                atomicMax(&last, i);
-            } else if ((double)r > want) {
-                atomicMin(&tok, i);
-                break;
+    const u64 sum = __shfl(inc, 63, 64), past = target(a, row, sum), t = thr;
+    const uint32_t g = __ffsll((unsigned long long)__ballot(inc > past)) - 1;
+    u64 run = __shfl(inc - mine, g, 64);
+    // ... and the token in it, 4096 words at a time
+    const uint32_t end = min(a.vocab, (g + 1) * a.part);
+    for (uint32_t i0 = g * a.part; i0 < end; i0 += 4096) {
+        const uint32_t i = i0 + 4 * tid;
+        float l[4];
+        u64 f[4], m = 0;
+        double v[4];
+        load4(a, x, i < end ? i : a.vocab, l);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const uint32_t b = bin_of(l[j], s);
+            f[j] = 0;
+            if (b < NB && (b < c.b_lo || (b <= c.b_hi && word(l[j], i + j) >= t))) {
+                v[j] = weight(l[j], s.top, a.inv_t);
+                if (v[j] >= (double)a.min_p || l[j] == s.top) f[j] = fixed(v[j]);
+            }
+            m += f[j];
+        }
+        u64 up = m;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const u64 q = __shfl_up(up, o, 64);
+            if (lane >= (uint32_t)o) up += q;
+        }
+        __syncthreads();
+        if (lane == 63) red[tid >> 6] = up;
+        __syncthreads();
+        u64 at = run + up - m;
+#pragma unroll
+        for (uint32_t k = 0; k < 16; k++) {
+            at += k < tid >> 6 ? red[k] : 0ull;
+            run += red[k];
+        }
+        if (at <= past && at + m > past) {
+            bool found = false;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                at += f[j];
+                if (!found && at > past) {
+                    found = true;
+                    emit(a, row, i + j, (float)(v[j] * ONE / (double)sum));
+                }
             }
         }
-    }
-    __syncthreads();
-    if (tid == 0) {
-        const uint32_t i = past ? last : tok;
-        emit(a, row, i, i < a.vocab ? (float)((double)kept_mass(i) / (double)sum) : 0.f);
+        if (run > past) break;
     }
 }
 
@@ -774,7 +885,11 @@ hipError_t launch_sample(const float *x, size_t ld, uint32_t rows, uint32_t voca
     w.n_list = (uint32_t *)(w.range + (size_t)rows * r.parts);
     const dim3 g(r.parts, rows);
     hipLaunchKernelGGL(k_range, g, dim3(256), 0, s, a, w);
-    if (a.k || a.top_p < 1.f) hipLaunchKernelGGL(k_hist, g, dim3(256), 0, s, a, w);
+    a.listed = a.k && a.k <= LIST / 2;
+    if (a.listed)
+        hipLaunchKernelGGL(k_hist<false>, g, dim3(256), 0, s, a, w);
+    else if (a.k || a.top_p < 1.f)
+        hipLaunchKernelGGL(k_hist<true>, g, dim3(256), 0, s, a, w);
     hipLaunchKernelGGL(k_collect, g, dim3(256), 0, s, a, w);
     hipLaunchKernelGGL(k_finish, dim3(rows), dim3(1024), 0, s, a, w);
     return hipGetLastError();
