@@ -35,7 +35,7 @@ typedef unsigned long long u64;
 
 constexpr uint32_t TK = 128;        // top_k of the first form
 constexpr uint32_t PICK_MAX = 8192; // words that a row's parts give it at most
-constexpr uint32_t NB = 2048;       // bins of the second form
+constexpr uint32_t NB = 1024;       // bins of the second form
 constexpr uint32_t LIST = 2048;     // words of the cuts' bins kept per row
 constexpr uint32_t MAX_PARTS = 256;  // of the first form; 64 of the second, one for each lane
 constexpr double ONE = 4398046511104.0;  // 2^42
@@ -113,6 +113,30 @@ __device__ __forceinline__ void load4(const Row &a, const float *x, uint32_t i, 
     }
 }
 
+// sums over the lanes up to and with each one (DPP moves: a shuffle goes through LDS)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_from(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_from(u64 x) {
+    return (u64)dpp_from<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | dpp_from<CTRL, ROWS>((uint32_t)x);
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T x) {
+    x += dpp_from<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: rows of sixteen
+    x += dpp_from<0x112, 0xf>(x);
+    x += dpp_from<0x114, 0xf>(x);
+    x += dpp_from<0x118, 0xf>(x);
+    x += dpp_from<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+    x += dpp_from<0x143, 0xc>(x);
+    return x;
+}
+__device__ __forceinline__ u64 lane_value(u64 x, uint32_t lane) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+
 // the token is the first word at which the running sum (of whole numbers) is
 // above this: floor(u sum), below sum itself
 __device__ __forceinline__ u64 target(const Row &a, uint32_t row, u64 sum) {
@@ -150,12 +174,12 @@ __device__ __forceinline__ uint32_t above(const u64 *list, uint32_t n, u64 w) {
     return r;
 }
 
-// The top_k words of a part (pieces g, g + parts, .. of 1024 words): word j of
-// part g in out[j][g], descending, zeros behind them.  The k-th largest of the 256
-// threads' own maxima bounds them from below, so that of a part's words little more
-// than k are ranked against one another.  The bound is of the logits alone (a
-// compare of 64 bits takes four times one of 32); where equal logits bring more
-// words to it than the list holds, of whole words: then at most k threads' all.
+// The top_k words of a part (a.part words, at most 1024 E): word j of part g in
+// out[j][g], descending, zeros behind them.  A logit that at least k of the 256
+// threads' own maxima reach bounds them from below, so that of a part's words little
+// more than k are ranked against one another.  Where equal logits bring more words
+// to it than the list holds, the bound is the k-th largest of the maxima as whole
+// words: then at most k threads' all.
 template <int E>
 __global__ __launch_bounds__(256) void k_part(Row a, u64 *__restrict__ out) {
     __shared__ __attribute__((aligned(16))) uint32_t best[256];
@@ -165,55 +189,72 @@ __global__ __launch_bounds__(256) void k_part(Row a, u64 *__restrict__ out) {
     __shared__ uint32_t cnt, low;
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y, k = a.k;
     const float *const x = a.x + row * a.ld;
+    const uint32_t first = g * a.part + 4 * tid, end = min(a.vocab, (g + 1) * a.part);
     float l[E][4];
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const size_t i = ((size_t)g + (size_t)a.parts * e) * 1024 + 4 * tid;
-        load4(a, x, (uint32_t)min(i, (size_t)a.vocab), l[e]);
-    }
+    for (int e = 0; e < E; e++) load4(a, x, first + 1024 * e < end ? first + 1024 * e : a.vocab, l[e]);
     if (tid == 0) low = 0xFFFFFFFFu, cnt = 0, thr = 1;
     uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < E; e++)
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) m = max(m, ord(l[e][j]));
+    // each wavefront's ceil(k / 4)-th largest maximum, by bits (down to a step of
+    // 2^-11 of it: a bound is enough); the least of the four is reached by k threads
+    // at least
+    uint32_t q = 0;
+#pragma unroll
+    for (int b = 31; b >= 12; b--) {
+        const uint32_t c = q | 1u << b;
+        if ((uint32_t)__popcll(__ballot(m >= c)) >= (k + 3) / 4) q = c;
+    }
     best[tid] = m;
     __syncthreads();
-    uint32_t r = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < 256; j += 32) {
-        u32x4 v[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = *reinterpret_cast<const u32x4 *>(best + j + 4 * e);
-#pragma unroll
-        for (int e = 0; e < 8; e++) r += (v[e][0] > m) + (v[e][1] > m) + (v[e][2] > m) + (v[e][3] > m);
-    }
-    // the least of the maxima that fewer than k exceed; 0 where there are fewer than k
-    if (r < k) atomicMin(&low, m);
+    if ((tid & 63) == 0) atomicMin(&low, q);
     __syncthreads();
-    const uint32_t lo = max(low, 1u);
+    if (low == 0) {
+        // a wavefront with fewer words: the least of all maxima that fewer than k exceed
+        uint32_t r = 0;
+#pragma unroll 1
+        for (uint32_t j = 0; j < 256; j += 32) {
+            u32x4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = *reinterpret_cast<const u32x4 *>(best + j + 4 * e);
+#pragma unroll
+            for (int e = 0; e < 8; e++) r += (v[e][0] > m) + (v[e][1] > m) + (v[e][2] > m) + (v[e][3] > m);
+        }
+        __syncthreads();
+        if (tid == 0) low = 0xFFFFFFFFu;
+        __syncthreads();
+        if (r < k) atomicMin(&low, m);
+        __syncthreads();
+    }
+    const uint32_t lo = max(low, 1u);  // 0 where there are fewer than k words
+    // the taken words to the list, one addition a wavefront for each of its words
     auto collect = [&](auto takes) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const uint32_t i = (g + a.parts * e) * 1024 + 4 * tid;
+            const uint32_t i = first + 1024 * e;
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
                 const u64 w = word(l[e][j], i + j);
-                if (takes(w)) {
-                    const uint32_t at = atomicAdd(&cnt, 1u);
-                    if (at < 4 * E * TK) list[at] = w;
-                }
+                const u64 who = __ballot(takes(w));
+                if (!who) continue;
+                uint32_t at = 0;
+                if ((tid & 63) == 0) at = atomicAdd(&cnt, (uint32_t)__popcll(who));
+                at = __builtin_amdgcn_readfirstlane(at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+                if (takes(w) && at < 4 * E * TK) list[at] = w;
             }
         }
     };
-    if (m >= lo) collect([&](u64 w) { return (uint32_t)(w >> 32) >= lo; });
+    collect([&](u64 w) { return (uint32_t)(w >> 32) >= lo; });
     __syncthreads();
     if (cnt > 4 * E * TK) {
         u64 mw = 0;
 #pragma unroll
         for (int e = 0; e < E; e++)
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) mw = max(mw, word(l[e][j], (g + a.parts * e) * 1024 + 4 * tid + j));
+            for (uint32_t j = 0; j < 4; j++) mw = max(mw, word(l[e][j], first + 1024 * e + j));
         bestw[tid] = mw;
         __syncthreads();
         if (tid == 0) cnt = 0;
@@ -265,8 +306,10 @@ __global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in)
     __syncthreads();
     u64 t = thr;
 #pragma unroll
-    for (uint32_t e = 0; e < PICK_MAX / 512; e++)
+    for (uint32_t e = 0; e < PICK_MAX / 512; e++) {
+        if (512 * e >= C) break;
         if (v[e] >= t) list[atomicAdd(&cnt, 1u)] = v[e];
+    }
     __syncthreads();
     uint32_t n = cnt;
     if (n > 1024) {
@@ -316,13 +359,8 @@ __global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in)
         p[e] = w[e] ? weight(word_logit(w[e]), top, a.inv_t) : 0.0;
         f[e] = fixed(p[e]);
     }
-    u64 inc = f[0] + f[1];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 x = __shfl_up(inc, o, 64);
-        if (tid >= (uint32_t)o) inc += x;
-    }
-    const double want = (double)a.top_p * (double)__shfl(inc, 63, 64);
+    const u64 inc = wave_scan(f[0] + f[1]);
+    const double want = (double)a.top_p * (double)lane_value(inc, 63);
     u64 before = inc - f[0] - f[1], sum = 0;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
@@ -333,8 +371,7 @@ __global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in)
         kept[2 * tid + e] = Kept{f[e], word_index(w[e]), 0};
     }
     if (tid < 4) kept[TK + tid] = Kept{0, 0, 0};
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    sum = lane_value(wave_scan(sum), 63);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // a word's sum in index order, over the kept words
     u64 upto[2] = {0, 0};
@@ -383,19 +420,23 @@ struct Work {
 
 __device__ __forceinline__ bool cuts(const Row &a) { return a.k || a.top_p < 1.f; }
 
-// f(logit, index) for the words of part g, by a workgroup of 256, sixteen words a
-// thread in flight
+// The words of part g for a workgroup of 256, four a thread at a time and the next
+// four in flight; f(logit, index), where words below `least` may be left out
 template <typename F>
-__device__ __forceinline__ void for_words(const Row &a, const float *x, uint32_t g, F f) {
+__device__ __forceinline__ void for_words(const Row &a, uint32_t row, uint32_t g, float least, F f) {
+    const float *const x = a.x + row * a.ld;
     const uint32_t end = min(a.vocab, (g + 1) * a.part);
-    for (uint32_t i0 = g * a.part + 4 * threadIdx.x; i0 < end; i0 += 4096) {
-        float l[4][4];
+    uint32_t i = g * a.part + 4 * threadIdx.x;
+    float l[4], n[4];
+    load4(a, x, i < end ? i : a.vocab, l);
+#pragma unroll 1
+    for (; i < end; i += 1024) {
+        load4(a, x, i + 1024 < end ? i + 1024 : a.vocab, n);
+        if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least)
 #pragma unroll
-        for (int e = 0; e < 4; e++) load4(a, x, i0 + 1024 * e < end ? i0 + 1024 * e : a.vocab, l[e]);
+            for (uint32_t j = 0; j < 4; j++) f(l[j], i + j);
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) f(l[e][j], i0 + 1024 * e + j);
+        for (int j = 0; j < 4; j++) l[j] = n[j];
     }
 }
 
@@ -407,7 +448,7 @@ __global__ __launch_bounds__(256) void k_range(Row a, Work w) {
         if (g == 0 && tid == 0) w.n_list[row] = 0;
     }
     uint32_t hi = 0, lo = 0xFFFFFFFFu;
-    for_words(a, a.x + row * a.ld, g, [&](float l, uint32_t) {
+    for_words(a, row, g, -INFINITY, [&](float l, uint32_t) {
         const uint32_t k = ord(l);
         hi = max(hi, k);
         lo = min(lo, k - 1);  // 0, never taken, is the largest
@@ -466,7 +507,7 @@ __global__ __launch_bounds__(256) void k_hist(Row a, Work w) {
     }
     const Scale s = row_scale(a, w, row);
     __syncthreads();
-    for_words(a, a.x + row * a.ld, g, [&](float l, uint32_t) {
+    for_words(a, row, g, -INFINITY, [&](float l, uint32_t) {
         const uint32_t b = bin_of(l, s);
         if (b == NB) return;
         if constexpr (MASS) {
@@ -498,14 +539,8 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
 #pragma unroll
     for (uint32_t i = 0; i < PER; i++) tm += m[i], tc += c[i];
     // exclusive sums of the threads' bins: within the wavefront, then over the four
-    u64 im = tm;
-    uint32_t ic = tc;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 vm = __shfl_up(im, o, 64);
-        const uint32_t vc = __shfl_up(ic, o, 64);
-        if ((tid & 63) >= (uint32_t)o) im += vm, ic += vc;
-    }
+    const u64 im = wave_scan(tm);
+    const uint32_t ic = wave_scan(tc);
     if ((tid & 63) == 63) ms[tid >> 6] = im, cs[tid >> 6] = ic;
     __syncthreads();
     u64 total = 0, pm = im - tm;
@@ -568,29 +603,65 @@ __device__ __forceinline__ bool in_cuts(uint32_t b, const Cut &c) { return b < N
 
 __global__ __launch_bounds__(256) void k_collect(Row a, Work w) {
     __shared__ u64 ms[5], put[LIST];
-    __shared__ uint32_t cs[4], base, cnt;
+    __shared__ uint32_t cs[4], base, cnt, got;
     __shared__ Cut cut;
     __shared__ u64 part[4];
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
     const Scale s = row_scale(a, w, row);
     Cut c = {NB, NB, NB, 0, 0, 0};
-    if (tid == 0) cnt = 0;
+    if (tid == 0) cnt = got = 0;
     if (cuts(a)) {
         c = find_cuts(a, w.hist[row], ms, cs, cut);
         if (g == 0 && tid == 0) w.cut[row] = c;
     }
     __syncthreads();
+    // Words below every bin that counts are passed over without their bin: a bin's
+    // logits are not below this (the second term covers the roundings of bin_of, of
+    // a bin's width, and of this difference)
+    float least = -INFINITY;
+    const uint32_t last = c.bk < NB ? c.bk : c.b_hi;
+    if (last < NB - 1 && s.inv > 0.f && s.top < INFINITY) {
+        const float d = (float)(last + 2) / s.inv;
+        least = s.top - d - 0x1p-20f * (fabsf(s.top) + d);
+    }
+    // the words of bins that count are gathered and then weighed all at once (one by
+    // one, every wavefront would wait for each of its few); too many go by in line
+    const uint32_t after = min(last + 1, NB);
     u64 sum = 0;
-    for_words(a, a.x + row * a.ld, g, [&](float l, uint32_t i) {
-        const uint32_t b = bin_of(l, s);
-        if (b < c.b_lo) {
-            const double v = weight(l, s.top, a.inv_t);
-            if (v >= (double)a.min_p || l == s.top) sum += fixed(v);
-        } else if (in_cuts(b, c)) {
-            const uint32_t at = atomicAdd(&cnt, 1u);
-            if (at < LIST) put[at] = word(l, i);
-        }
+    auto weigh = [&](float l) {
+        const double v = weight(l, s.top, a.inv_t);
+        if (v >= (double)a.min_p || l == s.top) sum += fixed(v);
+    };
+    for_words(a, row, g, least, [&](float l, uint32_t i) {
+        if (bin_of(l, s) >= after) return;
+        const uint32_t at = atomicAdd(&got, 1u);
+        if (at < LIST) put[at] = word(l, i);
     });
+    __syncthreads();
+    const uint32_t n = got;
+    __syncthreads();
+    if (n <= LIST) {
+        for (uint32_t i0 = 0; i0 < n; i0 += 256) {
+            const uint32_t i = i0 + tid;
+            const u64 v = i < n ? put[i] : 0ull;
+            const float l = word_logit(v);
+            const uint32_t b = i < n ? bin_of(l, s) : NB;
+            if (b < c.b_lo) weigh(l);
+            __syncthreads();  // put's first words make room for the list's
+            if (b >= c.b_lo && in_cuts(b, c)) put[atomicAdd(&cnt, 1u)] = v;
+            __syncthreads();
+        }
+    } else {
+        for_words(a, row, g, least, [&](float l, uint32_t i) {
+            const uint32_t b = bin_of(l, s);
+            if (b < c.b_lo) {
+                weigh(l);
+            } else if (in_cuts(b, c)) {
+                const uint32_t at = atomicAdd(&cnt, 1u);
+                if (at < LIST) put[at] = word(l, i);
+            }
+        });
+    }
     // the part's words behind those of other parts; a row with more than LIST
     // is counted in full and not read from the list
     __syncthreads();
@@ -598,9 +669,8 @@ __global__ __launch_bounds__(256) void k_collect(Row a, Work w) {
     __syncthreads();
     if (cnt)
         for (uint32_t i = tid; i < min(cnt, LIST) && base + i < LIST; i += 256) w.list[(size_t)row * LIST + base + i] = put[i];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if ((tid & 63) == 0) part[tid >> 6] = sum;
+    sum = wave_scan(sum);
+    if ((tid & 63) == 63) part[tid >> 6] = sum;
     __syncthreads();
     if (tid == 0) w.sum[(size_t)row * a.parts + g] = part[0] + part[1] + part[2] + part[3];
 }
@@ -608,10 +678,9 @@ __global__ __launch_bounds__(256) void k_collect(Row a, Work w) {
 // sum over the workgroup of 1024, in every thread
 template <typename T>
 __device__ __forceinline__ T wg_sum(T v, T (&sh)[16]) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    v = wave_scan(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     T r = 0;
 #pragma unroll
@@ -619,13 +688,33 @@ __device__ __forceinline__ T wg_sum(T v, T (&sh)[16]) {
     return r;
 }
 
+// size (1024 or 2048) words sorted, largest first, by a workgroup
+// of 1024: a bitonic network.  A pair no more than 64 apart is in its wavefront's
+// own 128 words, so that only the wider steps wait for the workgroup.
+__device__ __forceinline__ void sort_words(u64 *list, uint32_t size) {
+    const uint32_t t = threadIdx.x;
+    for (uint32_t k = 2; k <= size; k *= 2)
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+            if (2 * t < size) {
+                const uint32_t i = 2 * t - (t & (j - 1)), p = i + j;
+                const u64 x = list[i], y = list[p];
+                const bool down = (i & k) == 0 || k == size;
+                if (x < y == down) list[i] = y, list[p] = x;
+            }
+            if (j > 64 || (j == 1 && k >= 128))
+                __syncthreads();
+            else
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    __syncthreads();
+}
+
 // The cuts among the collected words, the kept words' sums by part, and the
 // token.  Where more words share the cuts' bins than the list holds (equal
 // logits by the thousand), the cuts are found bit by bit over the row itself.
 __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
-    __shared__ __attribute__((aligned(16))) u64 list[LIST + 8];
-    __shared__ __attribute__((aligned(16))) u64 wt[LIST + 8];  // weight; 0 where outside top-p's bins
-    __shared__ u64 part[64], red[16], thr_k, thr;
+    __shared__ __attribute__((aligned(16))) u64 list[LIST];
+    __shared__ u64 part[64], red[16], thr;
     __shared__ uint32_t redc[16];
     const uint32_t tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
     const float *const x = a.x + row * a.ld;
@@ -644,55 +733,61 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
         return;
     }
     if (tid < 64) part[tid] = tid < a.parts ? w.sum[(size_t)row * a.parts + tid] : 0ull;
-    if (tid == 0) thr_k = 0, thr = ~0ull;
+    if (tid == 0) thr = ~0ull;
     auto mass = [&](u64 v) { return fixed(weight(word_logit(v), s.top, a.inv_t)); };
     if (cut && n <= LIST) {
-        uint32_t in_bk = 0;
-        for (uint32_t i = tid; i < n; i += 1024) {
-            const u64 v = i < 1024 ? early : w.list[(size_t)row * LIST + i];
-            const uint32_t b = bin_of(word_logit(v), s);
-            list[i] = v;
-            wt[i] = b >= c.b_lo && b <= c.b_hi ? mass(v) : 0;
-            in_bk += b == c.bk;
-        }
-        if (tid < 8) list[n + tid] = 0, wt[n + tid] = 0;
-        u64 sk = c.before_k;
-        if (c.bk < NB) {
-            // the list's other words are of earlier bins, above bk's
-            const uint32_t last = n - wg_sum(in_bk, redc) + c.rank_k - 1;
-            for (uint32_t i = tid; i < n; i += 1024)
-                if (above(list, n, list[i]) == last) thr_k = list[i];
-        }
+        // sorted, largest first (zeros behind): a thread's words are two neighbours.  A
+        // few are ranked against one another, many go through the network
+        uint32_t size = 1024;
+        while (size < n) size *= 2;
+        for (uint32_t i = tid; i < size; i += 1024) list[i] = i >= n ? 0ull : i < 1024 ? early : w.list[(size_t)row * LIST + i];
         __syncthreads();
-        if (c.bk < NB || a.listed) {
-            u64 m = 0;
-            for (uint32_t i = tid; i < n; i += 1024)
-                if (list[i] >= thr_k && (a.listed || bin_of(word_logit(list[i]), s) == c.bk)) m += mass(list[i]);
-            sk += wg_sum(m, red);
+        if (n <= 512) {
+            const uint32_t rank = tid < n ? above(list, n, early) : 0;
+            __syncthreads();
+            if (tid < n) list[rank] = early;
+            __syncthreads();
+        } else {
+            sort_words(list, size);
         }
-        const double want = (double)a.top_p * (double)sk;
-        for (uint32_t i = tid; i < n; i += 1024) {
-            const u64 v = list[i];
-            const uint32_t b = bin_of(word_logit(v), s);
-            if (v < thr_k || b < c.b_lo || b > c.b_hi) continue;
-            if (a.top_p < 1.f) {
-                u64 before = c.before_lo;
-                for (uint32_t j = 0; j < n; j += 4) {
-                    u64x2 q[2], f[2];
+        u64 f[2] = {0, 0}, v[2] = {0, 0};
+        double wd[2] = {0.0, 0.0};
+        uint32_t b[2] = {NB, NB}, in_bk = 0;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        q[e] = *reinterpret_cast<const u64x2 *>(list + j + 2 * e);
-                        f[e] = *reinterpret_cast<const u64x2 *>(wt + j + 2 * e);
-                    }
+        for (int e = 0; e < 2; e++) {
+            if (2 * tid + e >= n) continue;
+            v[e] = list[2 * tid + e];
+            b[e] = bin_of(word_logit(v[e]), s);
+            wd[e] = weight(word_logit(v[e]), s.top, a.inv_t);
+            f[e] = fixed(wd[e]);
+            in_bk += b[e] == c.bk;
+        }
+        // top-k: the first rank_k of bk, before which are the list's words of earlier bins
+        const uint32_t keep_k = c.bk < NB ? n - wg_sum(in_bk, redc) + c.rank_k : n;
+        u64 m = 0;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) before += (q[e][0] > v ? f[e][0] : 0ull) + (q[e][1] > v ? f[e][1] : 0ull);
-                }
-                if (before && (double)before >= want) continue;
-            }
-            atomicMin(&thr, v);
-            const float l = word_logit(v);
-            if (l == s.top || weight(l, s.top, a.inv_t) >= (double)a.min_p)
-                atomicAdd(&part[word_index(v) / a.part], wt[i]);
+        for (int e = 0; e < 2; e++)
+            if (2 * tid + e < keep_k && (a.listed || b[e] == c.bk)) m += f[e];
+        const double want = (double)a.top_p * (double)(c.before_k + wg_sum(m, red));
+        // top-p: the words before which less than its share has been (its bins come
+        // first in the list)
+        const u64 up = wave_scan(f[0] + f[1]);
+        __syncthreads();
+        if (lane == 63) red[tid >> 6] = up;
+        __syncthreads();
+        u64 before = c.before_lo + up - f[0] - f[1];
+#pragma unroll
+        for (uint32_t k = 0; k < 16; k++) before += k < tid >> 6 ? red[k] : 0ull;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const bool keep = 2 * tid + e < keep_k && b[e] >= c.b_lo && b[e] <= c.b_hi && b[e] < NB &&
+                              (a.top_p >= 1.f || !before || (double)before < want);
+            before += f[e];
+            // the kept words are the first ones: the least of a wavefront's is its last
+            const u64 who = __ballot(keep);
+            if (!keep) continue;
+            if (lane == 63u - __clzll(who)) atomicMin(&thr, v[e]);
+            if (wd[e] == 1.0 || wd[e] >= (double)a.min_p) atomicAdd(&part[word_index(v[e]) / a.part], f[e]);
         }
         __syncthreads();
     } else if (cut) {
@@ -746,16 +841,10 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
         __syncthreads();
     }
     // the part that the token is in: every wavefront adds up the parts, one a lane
-    const u64 mine = part[lane];
-    u64 inc = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 v = __shfl_up(inc, o, 64);
-        if (lane >= (uint32_t)o) inc += v;
-    }
-    const u64 sum = __shfl(inc, 63, 64), past = target(a, row, sum), t = thr;
+    const u64 mine = part[lane], inc = wave_scan(mine);
+    const u64 sum = lane_value(inc, 63), past = target(a, row, sum), t = thr;
     const uint32_t g = __ffsll((unsigned long long)__ballot(inc > past)) - 1;
-    u64 run = __shfl(inc - mine, g, 64);
+    u64 run = lane_value(inc - mine, g);
     // ... and the token in it, 4096 words at a time
     const uint32_t end = min(a.vocab, (g + 1) * a.part);
     for (uint32_t i0 = g * a.part; i0 < end; i0 += 4096) {
@@ -774,12 +863,7 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
             }
             m += f[j];
         }
-        u64 up = m;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const u64 q = __shfl_up(up, o, 64);
-            if (lane >= (uint32_t)o) up += q;
-        }
+        const u64 up = wave_scan(m);
         __syncthreads();
         if (lane == 63) red[tid >> 6] = up;
         __syncthreads();
@@ -804,11 +888,13 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
     }
 }
 
-// parts of a row for the first form: pieces of 1024 words, E to a workgroup
-uint32_t part_pieces(uint32_t vocab, uint32_t *e) {
+// parts of a row for the first form: of one size, up to E pieces of 1024 words
+uint32_t part_pieces(uint32_t vocab, uint32_t *e, uint32_t *part) {
     const uint32_t pieces = (vocab + 1023) / 1024;
     *e = pieces <= 64 ? 1 : pieces <= 128 ? 2 : pieces <= 256 ? 4 : 8;
-    return (pieces + *e - 1) / *e;
+    const uint32_t g = (pieces + *e - 1) / *e;
+    *part = ((vocab + g - 1) / g + 3) / 4 * 4;
+    return (vocab + *part - 1) / *part;
 }
 // ... and for the second: about four workgroups per CU over all rows, each at
 // least 1024 words; a multiple of 4 words each, so that rows stay aligned
@@ -828,7 +914,7 @@ struct Plan {
 Plan plan(uint32_t rows, uint32_t vocab, const lrs_sampling &p) {
     Plan r = {};
     r.k = p.temperature == 0.f ? 1 : p.top_k >= vocab ? 0 : p.top_k;
-    r.parts = part_pieces(vocab, &r.e);
+    r.parts = part_pieces(vocab, &r.e, &r.part);
     r.first = r.k && r.k <= TK && r.parts <= MAX_PARTS && r.parts * r.k <= PICK_MAX;
     if (!r.first) r.parts = range_parts(vocab, rows, &r.part);
     return r;
