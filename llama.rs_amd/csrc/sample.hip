@@ -37,6 +37,7 @@ constexpr uint32_t TK = 128;        // top_k of the first form
 constexpr uint32_t PICK_MAX = 8192; // words that a row's parts give it at most
 constexpr uint32_t NB = 1024;       // bins of the second form
 constexpr uint32_t LIST = 2048;     // words of the cuts' bins kept per row
+constexpr uint32_t WG = 1024;       // threads of a workgroup of the second form: a part in one go where there is one row
 constexpr uint32_t MAX_PARTS = 256;  // of the first form; 64 of the second, one for each lane
 constexpr double ONE = 4398046511104.0;  // 2^42
 
@@ -306,10 +307,8 @@ __global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in)
     __syncthreads();
     u64 t = thr;
 #pragma unroll
-    for (uint32_t e = 0; e < PICK_MAX / 512; e++) {
-        if (512 * e >= C) break;
-        if (v[e] >= t) list[atomicAdd(&cnt, 1u)] = v[e];
-    }
+    for (uint32_t e = 0; e < PICK_MAX / 512; e++)
+        if (512 * e < C && v[e] >= t) list[atomicAdd(&cnt, 1u)] = v[e];
     __syncthreads();
     uint32_t n = cnt;
     if (n > 1024) {
@@ -361,14 +360,14 @@ __global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in)
     }
     const u64 inc = wave_scan(f[0] + f[1]);
     const double want = (double)a.top_p * (double)lane_value(inc, 63);
-    u64 before = inc - f[0] - f[1], sum = 0;
+    u64 before = inc - f[0] - f[1], sum = 0, kf[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         const bool keep = w[e] && ((tid == 0 && e == 0) || ((a.top_p >= 1.f || (double)before < want) && p[e] >= (double)a.min_p));
         before += f[e];
-        if (!keep) f[e] = 0;
-        sum += f[e];
-        kept[2 * tid + e] = Kept{f[e], word_index(w[e]), 0};
+        kf[e] = keep ? f[e] : 0ull;
+        sum += kf[e];
+        kept[2 * tid + e] = Kept{kf[e], word_index(w[e]), 0};
     }
     if (tid < 4) kept[TK + tid] = Kept{0, 0, 0};
     sum = lane_value(wave_scan(sum), 63);
@@ -388,12 +387,12 @@ __global__ __launch_bounds__(512) void k_pick(Row a, const u64 *__restrict__ in)
     }
     const u64 past = target(a, row, sum);
     uint32_t c = 0xFFFFFFFFu;
-    if (f[0] && upto[0] > past) c = i0;
-    if (f[1] && upto[1] > past) c = min(c, i1);
+    if (kf[0] && upto[0] > past) c = i0;
+    if (kf[1] && upto[1] > past) c = min(c, i1);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) c = min(c, (uint32_t)__shfl_xor(c, o, 64));
-    if (f[0] && i0 == c) emit(a, row, c, (float)(p[0] * ONE / (double)sum));
-    if (f[1] && i1 == c) emit(a, row, c, (float)(p[1] * ONE / (double)sum));
+    if (kf[0] && i0 == c) emit(a, row, c, (float)(p[0] * ONE / (double)sum));
+    if (kf[1] && i1 == c) emit(a, row, c, (float)(p[1] * ONE / (double)sum));
 }
 
 // ---- any top_k --------------------------------------------------------------
@@ -420,8 +419,8 @@ struct Work {
 
 __device__ __forceinline__ bool cuts(const Row &a) { return a.k || a.top_p < 1.f; }
 
-// The words of part g for a workgroup of 256, four a thread at a time and the next
-// four in flight; f(logit, index), where words below `least` may be left out
+// The words of part g, four a thread at a time and the next four in flight;
+// f(logit, index), where words below `least` may be left out
 template <typename F>
 __device__ __forceinline__ void for_words(const Row &a, uint32_t row, uint32_t g, float least, F f) {
     const float *const x = a.x + row * a.ld;
@@ -430,8 +429,8 @@ __device__ __forceinline__ void for_words(const Row &a, uint32_t row, uint32_t g
     float l[4], n[4];
     load4(a, x, i < end ? i : a.vocab, l);
 #pragma unroll 1
-    for (; i < end; i += 1024) {
-        load4(a, x, i + 1024 < end ? i + 1024 : a.vocab, n);
+    for (; i < end; i += 4 * WG) {
+        load4(a, x, i + 4 * WG < end ? i + 4 * WG : a.vocab, n);
         if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least)
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) f(l[j], i + j);
@@ -439,14 +438,27 @@ __device__ __forceinline__ void for_words(const Row &a, uint32_t row, uint32_t g
         for (int j = 0; j < 4; j++) l[j] = n[j];
     }
 }
+// sum over the workgroup, in every thread
+template <typename T>
+__device__ __forceinline__ T wg_sum(T v, T (&sh)[WG / 64]) {
+    v = wave_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    T r = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < WG / 64; i++) r += sh[i];
+    return r;
+}
 
-__global__ __launch_bounds__(256) void k_range(Row a, Work w) {
-    __shared__ uint32_t mx[4], mn[4];
+__global__ __launch_bounds__(WG) void k_range(Row a, Work w) {
+    __shared__ uint32_t mx, mn;
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
     if (cuts(a)) {
-        for (uint32_t i = g * 256 + tid; i < NB; i += a.parts * 256) w.hist[row].mass[i] = 0, w.hist[row].count[i] = 0;
+        for (uint32_t i = g * WG + tid; i < NB; i += a.parts * WG) w.hist[row].mass[i] = 0, w.hist[row].count[i] = 0;
         if (g == 0 && tid == 0) w.n_list[row] = 0;
     }
+    if (tid == 0) mx = 0, mn = 0xFFFFFFFFu;
     uint32_t hi = 0, lo = 0xFFFFFFFFu;
     for_words(a, row, g, -INFINITY, [&](float l, uint32_t) {
         const uint32_t k = ord(l);
@@ -458,11 +470,10 @@ __global__ __launch_bounds__(256) void k_range(Row a, Work w) {
         hi = max(hi, (uint32_t)__shfl_xor(hi, o, 64));
         lo = min(lo, (uint32_t)__shfl_xor(lo, o, 64));
     }
-    if ((tid & 63) == 0) mx[tid >> 6] = hi, mn[tid >> 6] = lo;
     __syncthreads();
-    if (tid == 0)
-        w.range[(size_t)row * a.parts + g] =
-            make_uint2(max(max(mx[0], mx[1]), max(mx[2], mx[3])), min(min(mn[0], mn[1]), min(mn[2], mn[3])) + 1);
+    if ((tid & 63) == 0) atomicMax(&mx, hi), atomicMin(&mn, lo);
+    __syncthreads();
+    if (tid == 0) w.range[(size_t)row * a.parts + g] = make_uint2(mx, mn + 1);
 }
 
 // the row's largest logit and the bins' scale, the same in every wavefront
@@ -496,15 +507,14 @@ __device__ __forceinline__ uint32_t bin_of(float l, const Scale &s) {
 
 // MASS: weights by bin too (not where the list will hold every word that counts)
 template <bool MASS>
-__global__ __launch_bounds__(256) void k_hist(Row a, Work w) {
+__global__ __launch_bounds__(WG) void k_hist(Row a, Work w) {
     __shared__ u64 mass[MASS ? NB : 1];
     __shared__ uint32_t count[NB];
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
     const bool counts = a.k != 0;
-    for (uint32_t i = tid; i < NB; i += 256) {
-        if constexpr (MASS) mass[i] = 0;
-        count[i] = 0;
-    }
+    static_assert(NB == WG, "a thread clears and adds a bin");
+    if constexpr (MASS) mass[tid] = 0;
+    count[tid] = 0;
     const Scale s = row_scale(a, w, row);
     __syncthreads();
     for_words(a, row, g, -INFINITY, [&](float l, uint32_t) {
@@ -518,35 +528,27 @@ __global__ __launch_bounds__(256) void k_hist(Row a, Work w) {
     });
     __syncthreads();
     Hist &h = w.hist[row];
-    for (uint32_t i = tid; i < NB; i += 256) {
-        if constexpr (MASS)
-            if (mass[i]) atomicAdd(&h.mass[i], mass[i]);
-        if (count[i]) atomicAdd(&h.count[i], count[i]);
-    }
+    if constexpr (MASS)
+        if (mass[tid]) atomicAdd(&h.mass[tid], mass[tid]);
+    if (count[tid]) atomicAdd(&h.count[tid], count[tid]);
 }
 
-// the bins of the cuts from the row's histogram, by a workgroup of 256
-__device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[5], uint32_t (&cs)[4], Cut &sh) {
-    constexpr uint32_t PER = NB / 256;
+// the bins of the cuts from the row's histogram, a bin a thread
+__device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[WG / 64], uint32_t (&cs)[WG / 64], u64 &after_k, Cut &sh) {
     const uint32_t tid = threadIdx.x;
-    u64 m[PER], tm = 0;
-    uint32_t c[PER], tc = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) {
-        m[i] = a.listed ? 0ull : h.mass[tid * PER + i];
-        c[i] = h.count[tid * PER + i];
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) tm += m[i], tc += c[i];
-    // exclusive sums of the threads' bins: within the wavefront, then over the four
-    const u64 im = wave_scan(tm);
-    const uint32_t ic = wave_scan(tc);
+    const u64 m = a.listed ? 0ull : h.mass[tid];
+    const uint32_t c = h.count[tid];
+    // sums of the bins before: within the wavefront, then over the wavefronts
+    const u64 im = wave_scan(m);
+    const uint32_t ic = wave_scan(c);
     if ((tid & 63) == 63) ms[tid >> 6] = im, cs[tid >> 6] = ic;
     __syncthreads();
-    u64 total = 0, pm = im - tm;
-    uint32_t n = 0, pc = ic - tc;
-    for (uint32_t i = 0; i < 4; i++) {
-        if (i < tid >> 6) pm += ms[i], pc += cs[i];
+    u64 total = 0, before = im - m;
+    uint32_t n = 0, nb = ic - c;
+#pragma unroll
+    for (uint32_t i = 0; i < WG / 64; i++) {
+        before += i < tid >> 6 ? ms[i] : 0ull;
+        nb += i < tid >> 6 ? cs[i] : 0u;
         total += ms[i];
         n += cs[i];
     }
@@ -555,22 +557,13 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
     if (tid == 0) {
         sh.b_lo = sh.b_hi = NB;
         sh.before_lo = 0;
-        if (!cut_k) sh.bk = NB, sh.rank_k = 0, sh.before_k = ms[4] = total;
+        if (!cut_k) sh.bk = NB, sh.rank_k = 0, sh.before_k = after_k = total;
     }
-    u64 bm = pm;
-    if (cut_k) {
-        uint32_t bc = pc;
-#pragma unroll
-        for (uint32_t i = 0; i < PER; i++) {
-            if (bc < a.k && bc + c[i] >= a.k) {
-                sh.bk = tid * PER + i;
-                sh.rank_k = a.k - bc;
-                sh.before_k = bm;
-                ms[4] = bm + m[i];
-            }
-            bc += c[i];
-            bm += m[i];
-        }
+    if (cut_k && nb < a.k && nb + c >= a.k) {
+        sh.bk = tid;
+        sh.rank_k = a.k - nb;
+        sh.before_k = before;
+        after_k = before + m;
     }
     __syncthreads();
     if (a.listed) {
@@ -578,16 +571,10 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
     } else if (a.top_p < 1.f) {
         // K's sum is between its sums before and after top-k's bin: top-p's cut is in
         // the bins that bring the sum to top_p times either
-        const double lo = (double)a.top_p * (double)sh.before_k, hi = (double)a.top_p * (double)ms[4];
-        bm = pm;
-#pragma unroll
-        for (uint32_t i = 0; i < PER; i++) {
-            const u64 nx = bm + m[i];
-            const bool first = tid * PER + i == 0;
-            if (((double)bm < lo || first) && (double)nx >= lo) sh.b_lo = tid * PER + i, sh.before_lo = bm;
-            if (((double)bm < hi || first) && (double)nx >= hi) sh.b_hi = tid * PER + i;
-            bm = nx;
-        }
+        const double lo = (double)a.top_p * (double)sh.before_k, hi = (double)a.top_p * (double)after_k;
+        const u64 nx = before + m;
+        if (((double)before < lo || tid == 0) && (double)nx >= lo) sh.b_lo = tid, sh.before_lo = before;
+        if (((double)before < hi || tid == 0) && (double)nx >= hi) sh.b_hi = tid;
     }
     __syncthreads();
     if (tid == 0 && !a.listed) {
@@ -601,17 +588,16 @@ __device__ __forceinline__ Cut find_cuts(const Row &a, const Hist &h, u64 (&ms)[
 
 __device__ __forceinline__ bool in_cuts(uint32_t b, const Cut &c) { return b < NB && ((b >= c.b_lo && b <= c.b_hi) || b == c.bk); }
 
-__global__ __launch_bounds__(256) void k_collect(Row a, Work w) {
-    __shared__ u64 ms[5], put[LIST];
-    __shared__ uint32_t cs[4], base, cnt, got;
+__global__ __launch_bounds__(WG) void k_collect(Row a, Work w) {
+    __shared__ u64 ms[WG / 64], put[LIST], after_k;
+    __shared__ uint32_t cs[WG / 64], base, cnt, got;
     __shared__ Cut cut;
-    __shared__ u64 part[4];
     const uint32_t tid = threadIdx.x, g = blockIdx.x, row = blockIdx.y;
     const Scale s = row_scale(a, w, row);
     Cut c = {NB, NB, NB, 0, 0, 0};
     if (tid == 0) cnt = got = 0;
     if (cuts(a)) {
-        c = find_cuts(a, w.hist[row], ms, cs, cut);
+        c = find_cuts(a, w.hist[row], ms, cs, after_k, cut);
         if (g == 0 && tid == 0) w.cut[row] = c;
     }
     __syncthreads();
@@ -641,7 +627,7 @@ __global__ __launch_bounds__(256) void k_collect(Row a, Work w) {
     const uint32_t n = got;
     __syncthreads();
     if (n <= LIST) {
-        for (uint32_t i0 = 0; i0 < n; i0 += 256) {
+        for (uint32_t i0 = 0; i0 < n; i0 += WG) {
             const uint32_t i = i0 + tid;
             const u64 v = i < n ? put[i] : 0ull;
             const float l = word_logit(v);
@@ -668,28 +654,13 @@ __global__ __launch_bounds__(256) void k_collect(Row a, Work w) {
     if (tid == 0 && cnt) base = atomicAdd(&w.n_list[row], cnt);
     __syncthreads();
     if (cnt)
-        for (uint32_t i = tid; i < min(cnt, LIST) && base + i < LIST; i += 256) w.list[(size_t)row * LIST + base + i] = put[i];
-    sum = wave_scan(sum);
-    if ((tid & 63) == 63) part[tid >> 6] = sum;
-    __syncthreads();
-    if (tid == 0) w.sum[(size_t)row * a.parts + g] = part[0] + part[1] + part[2] + part[3];
-}
-
-// sum over the workgroup of 1024, in every thread
-template <typename T>
-__device__ __forceinline__ T wg_sum(T v, T (&sh)[16]) {
-    v = wave_scan(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    T r = 0;
-#pragma unroll
-    for (int i = 0; i < 16; i++) r += sh[i];
-    return r;
+        for (uint32_t i = tid; i < min(cnt, LIST) && base + i < LIST; i += WG) w.list[(size_t)row * LIST + base + i] = put[i];
+    sum = wg_sum(sum, ms);
+    if (tid == 0) w.sum[(size_t)row * a.parts + g] = sum;
 }
 
 // size (1024 or 2048) words sorted, largest first, by a workgroup
-// of 1024: a bitonic network.  A pair no more than 64 apart is in its wavefront's
+// of WG: a bitonic network.  A pair no more than 64 apart is in its wavefront's
 // own 128 words, so that only the wider steps wait for the workgroup.
 __device__ __forceinline__ void sort_words(u64 *list, uint32_t size) {
     const uint32_t t = threadIdx.x;
@@ -709,13 +680,37 @@ __device__ __forceinline__ void sort_words(u64 *list, uint32_t size) {
     __syncthreads();
 }
 
+// n of list's words (up to LIST) sorted, largest first: a few are ranked against one
+// another, many go through the network
+__device__ __forceinline__ void order_words(u64 *list, uint32_t n) {
+    const uint32_t tid = threadIdx.x;
+    if (n <= 512) {
+        if (tid < 8) list[n + tid] = 0;
+        __syncthreads();
+        const u64 v = tid < n ? list[tid] : 0ull;
+        const uint32_t rank = tid < n ? above(list, n, v) : 0;
+        __syncthreads();
+        if (tid < n) list[rank] = v;
+        __syncthreads();
+    } else {
+        const uint32_t size = n <= 1024 ? 1024 : 2048;
+        for (uint32_t i = n + tid; i < size; i += WG) list[i] = 0;
+        __syncthreads();
+        sort_words(list, size);
+    }
+}
+
 // The cuts among the collected words, the kept words' sums by part, and the
-// token.  Where more words share the cuts' bins than the list holds (equal
-// logits by the thousand), the cuts are found bit by bit over the row itself.
-__global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
-    __shared__ __attribute__((aligned(16))) u64 list[LIST];
-    __shared__ u64 part[64], red[16], thr;
-    __shared__ uint32_t redc[16];
+// token.  Only the words of the bins that the cuts fall in are ordered.  Where more
+// of them than the list holds share those bins (equal logits by the thousand), the
+// cuts are found bit by bit over the row itself.
+__global__ __launch_bounds__(WG) void k_finish(Row a, Work w) {
+    __shared__ __attribute__((aligned(16))) u64 list[LIST + 8];
+    __shared__ u64 mass_of[NB];
+    __shared__ uint32_t cnt, bin_p;
+    __shared__ u64 before_p;
+    __shared__ u64 part[64], red[WG / 64], thr;
+    __shared__ uint32_t redc[WG / 64];
     const uint32_t tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
     const float *const x = a.x + row * a.ld;
     const bool cut = cuts(a);
@@ -736,59 +731,130 @@ __global__ __launch_bounds__(1024) void k_finish(Row a, Work w) {
     if (tid == 0) thr = ~0ull;
     auto mass = [&](u64 v) { return fixed(weight(word_logit(v), s.top, a.inv_t)); };
     if (cut && n <= LIST) {
-        // sorted, largest first (zeros behind): a thread's words are two neighbours.  A
-        // few are ranked against one another, many go through the network
-        uint32_t size = 1024;
-        while (size < n) size *= 2;
-        for (uint32_t i = tid; i < size; i += 1024) list[i] = i >= n ? 0ull : i < 1024 ? early : w.list[(size_t)row * LIST + i];
-        __syncthreads();
-        if (n <= 512) {
-            const uint32_t rank = tid < n ? above(list, n, early) : 0;
-            __syncthreads();
-            if (tid < n) list[rank] = early;
-            __syncthreads();
-        } else {
-            sort_words(list, size);
-        }
-        u64 f[2] = {0, 0}, v[2] = {0, 0};
+        u64 v[2], f[2] = {0, 0}, thr_k = 0;
         double wd[2] = {0.0, 0.0};
-        uint32_t b[2] = {NB, NB}, in_bk = 0;
+        uint32_t b[2] = {NB, NB};
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            if (2 * tid + e >= n) continue;
-            v[e] = list[2 * tid + e];
+            const uint32_t i = tid + WG * e;
+            v[e] = i >= n ? 0ull : e == 0 ? early : w.list[(size_t)row * LIST + i];
+            if (!v[e]) continue;
             b[e] = bin_of(word_logit(v[e]), s);
             wd[e] = weight(word_logit(v[e]), s.top, a.inv_t);
             f[e] = fixed(wd[e]);
-            in_bk += b[e] == c.bk;
         }
-        // top-k: the first rank_k of bk, before which are the list's words of earlier bins
-        const uint32_t keep_k = c.bk < NB ? n - wg_sum(in_bk, redc) + c.rank_k : n;
-        u64 m = 0;
+        // the words that `takes` says, in order
+        auto gather = [&](auto takes) __attribute__((always_inline)) {
+            __syncthreads();
+            if (tid == 0) cnt = 0;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                if (takes(e)) list[atomicAdd(&cnt, 1u)] = v[e];
+            __syncthreads();
+            const uint32_t m = cnt;
+            order_words(list, m);
+            return m;
+        };
+        if (c.bk < NB) {
+            gather([&](int e) { return b[e] == c.bk; });
+            thr_k = list[c.rank_k - 1];
+        }
+        auto in_k = [&](int e) { return v[e] && v[e] >= thr_k; };
+        if (a.top_p < 1.f) {
+            u64 m = 0;
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                if (in_k(e) && (a.listed || b[e] == c.bk)) m += f[e];
+            const double want = (double)a.top_p * (double)(c.before_k + wg_sum(m, red));
+            if (a.listed) {
+                // the bin that the cut is in, from these words' weights by bin
+                mass_of[tid] = 0;
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (in_k(e)) atomicAdd(&mass_of[b[e]], f[e]);
+                __syncthreads();
+                const u64 mine = mass_of[tid], up = wave_scan(mine);
+                if (lane == 63) red[tid >> 6] = up;
+                __syncthreads();
+                u64 before = up - mine;
+#pragma unroll
+                for (uint32_t k = 0; k < WG / 64; k++) before += k < tid >> 6 ? red[k] : 0ull;
+                if (((double)before < want || tid == 0) && (double)(before + mine) >= want) bin_p = tid, before_p = before;
+                __syncthreads();
+                c.b_lo = c.b_hi = bin_p;
+                c.before_lo = before_p;
+            }
+            const uint32_t sub = gather([&](int e) { return in_k(e) && b[e] >= c.b_lo && b[e] <= c.b_hi; });
+            // the words before which less than top-p's share has been, two a thread
+            u64 x[2], g[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                x[e] = 2 * tid + e < sub ? list[2 * tid + e] : 0ull;
+                g[e] = x[e] ? mass(x[e]) : 0ull;
+            }
+            const u64 up = wave_scan(g[0] + g[1]);
+            if (lane == 63) red[tid >> 6] = up;
+            __syncthreads();
+            u64 before = c.before_lo + up - g[0] - g[1];
+#pragma unroll
+            for (uint32_t k = 0; k < WG / 64; k++) before += k < tid >> 6 ? red[k] : 0ull;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const bool keep = x[e] && (!before || (double)before < want);
+                before += g[e];
+                // they are the first ones: the least of a wavefront's is its last
+                const u64 who = __ballot(keep);
+                if (keep && lane == 63u - __clzll(who)) atomicMin(&thr, x[e]);
+            }
+        } else if (tid == 0) {
+            thr = thr_k ? thr_k : 1;
+        }
+        __syncthreads();
+        const u64 t = thr;
+        if (a.listed) {
+            // every kept word is here: their sums by index, NB stretches of the vocabulary,
+            // the stretch that the token is in, and the token among its words
+            mass_of[tid] = 0;
+            __syncthreads();
+            const uint32_t span = (a.vocab + NB - 1) / NB;
+            u64 kf[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const bool kept = v[e] && (b[e] < c.b_lo || (b[e] <= c.b_hi && v[e] >= t)) && (wd[e] == 1.0 || wd[e] >= (double)a.min_p);
+                kf[e] = kept ? f[e] : 0ull;
+                if (kf[e]) atomicAdd(&mass_of[word_index(v[e]) / span], kf[e]);
+            }
+            __syncthreads();
+            const u64 mine = mass_of[tid], up = wave_scan(mine);
+            if (lane == 63) red[tid >> 6] = up;
+            __syncthreads();
+            u64 at = up - mine, sum = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < WG / 64; k++) {
+                at += k < tid >> 6 ? red[k] : 0ull;
+                sum += red[k];
+            }
+            const u64 past = target(a, row, sum);
+            if (at <= past && at + mine > past) bin_p = tid, before_p = at;
+            __syncthreads();
+            const uint32_t stretch = bin_p;
+            const u64 before = before_p;
+            const uint32_t m = gather([&](int e) { return kf[e] && word_index(v[e]) / span == stretch; });
+            for (uint32_t i = tid; i < m; i += WG) {
+                const uint32_t index = word_index(list[i]);
+                u64 r = before;
+                for (uint32_t j = 0; j < m; j++) r += word_index(list[j]) < index ? mass(list[j]) : 0ull;
+                const double wi = weight(word_logit(list[i]), s.top, a.inv_t);
+                if (r <= past && r + fixed(wi) > past) emit(a, row, index, (float)(wi * ONE / (double)sum));
+            }
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < 2; e++)
-            if (2 * tid + e < keep_k && (a.listed || b[e] == c.bk)) m += f[e];
-        const double want = (double)a.top_p * (double)(c.before_k + wg_sum(m, red));
-        // top-p: the words before which less than its share has been (its bins come
-        // first in the list)
-        const u64 up = wave_scan(f[0] + f[1]);
-        __syncthreads();
-        if (lane == 63) red[tid >> 6] = up;
-        __syncthreads();
-        u64 before = c.before_lo + up - f[0] - f[1];
-#pragma unroll
-        for (uint32_t k = 0; k < 16; k++) before += k < tid >> 6 ? red[k] : 0ull;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const bool keep = 2 * tid + e < keep_k && b[e] >= c.b_lo && b[e] <= c.b_hi && b[e] < NB &&
-                              (a.top_p >= 1.f || !before || (double)before < want);
-            before += f[e];
-            // the kept words are the first ones: the least of a wavefront's is its last
-            const u64 who = __ballot(keep);
-            if (!keep) continue;
-            if (lane == 63u - __clzll(who)) atomicMin(&thr, v[e]);
-            if (wd[e] == 1.0 || wd[e] >= (double)a.min_p) atomicAdd(&part[word_index(v[e]) / a.part], f[e]);
-        }
+            if (v[e] && (b[e] < c.b_lo || (b[e] <= c.b_hi && v[e] >= t)) && (wd[e] == 1.0 || wd[e] >= (double)a.min_p))
+                atomicAdd(&part[word_index(v[e]) / a.part], f[e]);
         __syncthreads();
     } else if (cut) {
         // bit by bit the largest value that enough of the bins' words reach
@@ -896,11 +962,13 @@ uint32_t part_pieces(uint32_t vocab, uint32_t *e, uint32_t *part) {
     *part = ((vocab + g - 1) / g + 3) / 4 * 4;
     return (vocab + *part - 1) / *part;
 }
-// ... and for the second: about four workgroups per CU over all rows, each at
-// least 1024 words; a multiple of 4 words each, so that rows stay aligned
-uint32_t range_parts(uint32_t vocab, uint32_t rows, uint32_t *part) {
+// ... and for the second: a workgroup per CU over all rows, four where k_finish
+// goes over a part again (64 rows of 248320 words with top_k 1000 in 4, 8, 16 parts a
+// row: k_collect 19, 24, 36 us); each at least 1024 words, a multiple of 4, so that
+// rows stay aligned
+uint32_t range_parts(uint32_t vocab, uint32_t rows, bool listed, uint32_t *part) {
     const uint32_t pieces = (vocab + 1023) / 1024;
-    uint32_t g = (1024 + rows - 1) / rows;
+    uint32_t g = ((listed ? 256 : 1024) + rows - 1) / rows;
     g = g < 4 ? 4 : g > 64 ? 64 : g;
     if (g > pieces) g = pieces;
     *part = ((vocab + g - 1) / g + 3) / 4 * 4;
@@ -908,7 +976,7 @@ uint32_t range_parts(uint32_t vocab, uint32_t rows, uint32_t *part) {
 }
 
 struct Plan {
-    bool first;
+    bool first, listed;
     uint32_t e, parts, part, k;
 };
 Plan plan(uint32_t rows, uint32_t vocab, const lrs_sampling &p) {
@@ -916,7 +984,8 @@ Plan plan(uint32_t rows, uint32_t vocab, const lrs_sampling &p) {
     r.k = p.temperature == 0.f ? 1 : p.top_k >= vocab ? 0 : p.top_k;
     r.parts = part_pieces(vocab, &r.e, &r.part);
     r.first = r.k && r.k <= TK && r.parts <= MAX_PARTS && r.parts * r.k <= PICK_MAX;
-    if (!r.first) r.parts = range_parts(vocab, rows, &r.part);
+    r.listed = !r.first && r.k && r.k <= LIST / 2;
+    if (!r.first) r.parts = range_parts(vocab, rows, r.listed, &r.part);
     return r;
 }
 
@@ -970,14 +1039,14 @@ hipError_t launch_sample(const float *x, size_t ld, uint32_t rows, uint32_t voca
     w.range = (uint2 *)(w.sum + (size_t)rows * r.parts);
     w.n_list = (uint32_t *)(w.range + (size_t)rows * r.parts);
     const dim3 g(r.parts, rows);
-    hipLaunchKernelGGL(k_range, g, dim3(256), 0, s, a, w);
-    a.listed = a.k && a.k <= LIST / 2;
+    hipLaunchKernelGGL(k_range, g, dim3(WG), 0, s, a, w);
+    a.listed = r.listed;
     if (a.listed)
-        hipLaunchKernelGGL(k_hist<false>, g, dim3(256), 0, s, a, w);
+        hipLaunchKernelGGL(k_hist<false>, g, dim3(WG), 0, s, a, w);
     else if (a.k || a.top_p < 1.f)
-        hipLaunchKernelGGL(k_hist<true>, g, dim3(256), 0, s, a, w);
-    hipLaunchKernelGGL(k_collect, g, dim3(256), 0, s, a, w);
-    hipLaunchKernelGGL(k_finish, dim3(rows), dim3(1024), 0, s, a, w);
+        hipLaunchKernelGGL(k_hist<true>, g, dim3(WG), 0, s, a, w);
+    hipLaunchKernelGGL(k_collect, g, dim3(WG), 0, s, a, w);
+    hipLaunchKernelGGL(k_finish, dim3(rows), dim3(WG), 0, s, a, w);
     return hipGetLastError();
 }
 
