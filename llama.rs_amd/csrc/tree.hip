@@ -136,6 +136,8 @@ hipError_t launch_rope_append(const RopeAppend &a, hipStream_t s) {
 // The subtracted maximum follows the scores only when one exceeds it by 2^8: then
 // the sums are rescaled; p stays below 2^8, which f32 sums and f16 pairs hold.
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
 typedef __fp16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __fp16 h16x4_t __attribute__((ext_vector_type(4)));
@@ -221,7 +223,15 @@ __global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(
             __builtin_amdgcn_global_load_lds(vb + at + 8 * (pc ^ ((row >> VT & VM) << 2)), (lds_void_t *)((odd ? buf1[grp] : buf0[grp]) + 32 * HD + 512 * j), 16, 0, 0);
         }
     };
+    // the same rounds for every group; the first `plain` of them are of positions
+    // that every row sees.  The two buffers are objects of their own and the
+    // plain rounds' parity is fixed, so that the compiler need not wait for the
+    // loads into one before it reads the other
     const uint32_t first = c0 + grp;
+    const uint32_t rounds = c1 > c0 ? (c1 - c0 + G - 1) / G : 0, whole = min(c1, a.len / 32);
+    const uint32_t plain = whole > c0 ? (whole - c0) / G : 0;
+    // what the row sees of its masked chunk: read a round ahead
+    uint32_t seen = seen_bits(a, node, first + (plain & ~1u) * G);
     f16x8_t qh[KS], ql[KS];
     float qsc;
     {
@@ -265,11 +275,11 @@ __global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(
 #pragma unroll
         for (int i = 0; i < 16; i++) o[t][i] = 0.f;
     float m = -INFINITY, l = 0.f;  // l: of the lane's own positions
-    // the products of chunk c in buffer b; masked (a constant): it has positions that some
-    // rows do not see
-    auto chunk = [&](const bool masked, uint32_t c, const _Float16 *b) __attribute__((always_inline)) {
+    // the products of the chunk in buffer b; masked (a constant): it has positions that some
+    // rows do not see, the row's are `seen`
+    auto chunk = [&](const bool masked, uint32_t seen, const _Float16 *b) __attribute__((always_inline)) {
         const _Float16 *const Kc = b, *const Vc = b + 32 * HD;
-        const uint32_t mine = masked ? seen_bits(a, node, c) >> (4 * hf) : 0xFFFFFFFFu;
+        const uint32_t mine = seen >> (4 * hf);
         f32x16_t sc;
 #pragma unroll
         for (int i = 0; i < 16; i++) sc[i] = 0.f;
@@ -329,37 +339,43 @@ __global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(
             // a V that is not finite reaches the rows that see it alone: it is taken
             // out of the product (0 inf is NaN) and added where it is seen
             if (masked) {
-                f16x8_t one;
+                u16x2_t top = {0, 0};
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    one[j] = mine >> (16 * s + 8 * (j >> 2) + (j & 3)) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+                for (int t = 0; t < OT; t++)
 #pragma unroll
-                for (int t = 0; t < OT; t++) {
-                    bool odd = false;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) odd |= !(__builtin_fabsf16(va[t][j]) <= (_Float16)65504.0f);
-                    if (!__any(odd)) continue;
-#pragma unroll 1
-                    for (int kind = 0; kind < 3; kind++) {  // NaN, inf, -inf
-                        f16x8_t is;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const _Float16 v = va[t][j];
-                            const bool hit = kind == 0 ? v != v : v == (kind == 1 ? (_Float16)INFINITY : -(_Float16)INFINITY);
-                            is[j] = hit ? (_Float16)1.0f : (_Float16)0.0f;
-                        }
-                        f32x16_t n;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) n[i] = 0.f;
-                        n = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, one, n, 0, 0, 0);
-                        const float val = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (n[i] > 0.f) o[t][i] += val;
+                    for (int j = 0; j < 8; j += 2) {
+                        const u16x8_t bits = __builtin_bit_cast(u16x8_t, va[t]) & (uint16_t)0x7FFF;
+                        top = __builtin_elementwise_max(top, u16x2_t{bits[j], bits[j + 1]});
                     }
+                if (__any(max(top[0], top[1]) >= 0x7C00)) {
+                    f16x8_t one;
 #pragma unroll
                     for (int j = 0; j < 8; j++)
-                        if (!(__builtin_fabsf16(va[t][j]) <= (_Float16)65504.0f)) va[t][j] = (_Float16)0.0f;
+                        one[j] = mine >> (16 * s + 8 * (j >> 2) + (j & 3)) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+                    for (int t = 0; t < OT; t++) {
+#pragma unroll 1
+                        for (int kind = 0; kind < 3; kind++) {  // NaN, inf, -inf
+                            f16x8_t is;
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                const _Float16 v = va[t][j];
+                                const bool hit = kind == 0 ? v != v : v == (kind == 1 ? (_Float16)INFINITY : -(_Float16)INFINITY);
+                                is[j] = hit ? (_Float16)1.0f : (_Float16)0.0f;
+                            }
+                            f32x16_t n;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) n[i] = 0.f;
+                            n = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, one, n, 0, 0, 0);
+                            const float val = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                if (n[i] > 0.f) o[t][i] += val;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (!(__builtin_fabsf16(va[t][j]) <= (_Float16)65504.0f)) va[t][j] = (_Float16)0.0f;
+                    }
                 }
             }
             // neighbouring products go to different sums
@@ -369,12 +385,6 @@ __global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(
             for (int t = 0; t < OT; t++) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[t], ph[s], o[t], 0, 0, 0);
         }
     };
-    // the same rounds for every group; the first `plain` of them are of positions
-    // that every row sees.  The two buffers are objects of their own and the
-    // plain rounds' parity is fixed, so that the compiler need not wait for the
-    // loads into one before it reads the other
-    const uint32_t rounds = c1 > c0 ? (c1 - c0 + G - 1) / G : 0, whole = min(c1, a.len / 32);
-    const uint32_t plain = whole > c0 ? (whole - c0) / G : 0;
     auto next = [&](uint32_t it, const bool odd) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
@@ -383,13 +393,15 @@ __global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(
     uint32_t it = 0;
     for (; it + 1 < plain; it += 2) {
         next(it, false);
-        chunk(false, first + it * G, buf0[grp]);
+        chunk(false, 0xFFFFFFFFu, buf0[grp]);
         next(it + 1, true);
-        chunk(false, first + (it + 1) * G, buf1[grp]);
+        chunk(false, 0xFFFFFFFFu, buf1[grp]);
     }
     for (; it < rounds; it++) {
+        const uint32_t c = first + it * G, now = seen;
         next(it, it & 1);
-        if (first + it * G < c1) chunk(true, first + it * G, it & 1 ? buf1[grp] : buf0[grp]);
+        seen = seen_bits(a, node, c + G);
+        if (c < c1) chunk(true, now, it & 1 ? buf1[grp] : buf0[grp]);
     }
     l += __shfl_xor(l, 32, 64);
     float M = m, L = l, f = 1.f;
@@ -440,7 +452,7 @@ __global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(
 #pragma unroll
         for (int w = 0; w < G; w++) {
             const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(q < 32 ? buf0[w] : buf1[w]) +
-                                                               (q % 32) * HD + 4 * (d ^ (q % (HD / 4))));
+                                                               (q % 32) * HD + 4 * (d ^ (q % 32 % (HD / 4))));
             v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         }
         *reinterpret_cast<float4 *>(out + ((size_t)(row / rep) * a.n_head + g * rep + row % rep) * HD + 4 * d) = v;
