@@ -421,11 +421,14 @@ int lrs_decode_greedy(lrs_model *m, uint32_t token, uint32_t pos, uint32_t *next
  * on the device with no host round trip per token (out_tokens[n_gen]). */
 int lrs_generate_greedy(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uint32_t pos0,
                         uint32_t n_gen, uint32_t *out_tokens);
-/* decode + sampling on the device (lrs_sample_dev's rule, u in [0, 1)).  A row
- * of logits without a word that can be taken fails with LRS_E_HIP. */
+/* decode + sampling on the device (lrs_sample_dev's rule, u in [0, 1)).  Logits
+ * without a word that can be taken fail with LRS_E_HIP; `token` is cached then,
+ * as after lrs_decode. */
 int lrs_decode_sample(lrs_model *m, uint32_t token, uint32_t pos, const lrs_sampling *p, float u, uint32_t *next);
 /* lrs_generate_greedy with every token sampled: token i of out_tokens[n_gen]
- * from u[i], with no host round trip per token. */
+ * from u[i], with no host round trip per token.  Where a token cannot be
+ * sampled (LRS_E_HIP) the cache ends behind the tokens before it; a hybrid
+ * model is reset. */
 int lrs_generate_sample(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uint32_t pos0, uint32_t n_gen,
                         const lrs_sampling *p, const float *u, uint32_t *out_tokens);
 /* A tree of n drafted tokens in one pass over the weights (dense models whose
@@ -447,7 +450,8 @@ int lrs_tree_keep(lrs_model *m, const uint32_t *nodes, uint32_t n_nodes);
  * node.  out_tokens[n]: the n_out tokens of that walk (1 at least), of which all
  * but the last are cached with node 0's; the last is the next root.  Rejected
  * rows are dropped.  A sampled token that no child drafted still counts, so the
- * tokens are distributed as those of lrs_decode_sample. */
+ * tokens are distributed as those of lrs_decode_sample.  Where a token of the
+ * walk cannot be sampled (LRS_E_HIP) the cache ends at pos0. */
 int lrs_verify_tree(lrs_model *m, const uint32_t *tokens, const uint32_t *parents, uint32_t n, uint32_t pos0,
                     const lrs_sampling *p, const float *u, uint32_t *out_tokens, uint32_t *n_out);
 /* Per-op timing of the decode plan (the LLAMA_RS_PROFILE timestamps of

@@ -734,10 +734,6 @@ int lrs_attn_tree_dev(lrs_ctx *ctx, const lrs_kv *kv, const float *q_dev, uint32
     return LRS_OK;
 }
 
-}  // extern "C"
-
-extern "C" {
-
 // ---- graph capture of the asynchronous (*_dev) entry points ----
 struct lrs_graph {
     lrs_ctx *ctx;

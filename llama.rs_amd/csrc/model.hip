@@ -1736,7 +1736,13 @@ static int generate(lrs_model *m, const uint32_t *prompt, uint32_t n_prompt, uin
     memcpy(out_tokens, m->gen_host, n_gen * sizeof(uint32_t));
     if (p)
         for (uint32_t i = 0; i < n_gen; i++)
-            if (out_tokens[i] == LRS_NO_TOKEN) return fail(LRS_E_HIP, "no word of the logits can be sampled");
+            if (out_tokens[i] == LRS_NO_TOKEN) {
+                // cached: the prompt and the tokens before; a recurrent state has
+                // gone past them
+                m->len = pos0 + n_prompt + i;
+                if (m->hybrid) lrs_reset(m);
+                return fail(LRS_E_HIP, "no word of the logits can be sampled");
+            }
     m->len = pos0 + n_prompt + n_gen - 1;
     return LRS_OK;
 }
@@ -1773,9 +1779,9 @@ int lrs_decode_sample(lrs_model *m, uint32_t token, uint32_t pos, const lrs_samp
     LRS_HIP(publish(m, m->step, m->words_host, 1));
     LRS_HIP(hipStreamSynchronize(s));
     if (int e = ao_err_check(m)) return e;
+    m->len = pos + 1;
     if (m->words_host[0] == LRS_NO_TOKEN) return fail(LRS_E_HIP, "no word of the logits can be sampled");
     *next = m->words_host[0];
-    m->len = pos + 1;
     return LRS_OK;
 }
 
@@ -1933,6 +1939,7 @@ int lrs_model_profile(lrs_model *m, uint32_t op, uint32_t iters, float *avg_us, 
     for (uint32_t l = 0; l < c.n_layer; l++)
         if ((!dn_op && !attn_op) || (dn_op == m->layers[l].dn)) ls.push_back(l);
     if (ls.empty()) return fail(LRS_E_ARG, "no layer of this kind");
+    m->tree_n = 0;
     LRS_HIP(hipSetDevice(m->ctx->device));
     hipStream_t s = m->ctx->stream;
     const bool per_layer = op != LRS_OP_HEAD;

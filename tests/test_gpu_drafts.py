@@ -113,6 +113,43 @@ def test_sample_equal_words_past_the_list(lrs, ctx):
         check_rows(tok, prob, x, u, opt)
 
 
+@pytest.mark.parametrize("opt", [dict(top_k=129), dict(top_k=500), dict(top_k=500, top_p=0.5), dict(top_k=1024, min_p=0.5),
+                                 dict(top_k=1024, top_p=0.9, min_p=0.01), dict(top_k=1025, top_p=0.9)],
+                         ids=lambda o: "-".join(f"{k[-1]}{v}" for k, v in o.items()))
+def test_sample_equal_words_around_a_rank(lrs, ctx, opt):
+    """the last kept rank among more equal words than a row's list holds, and among fewer"""
+    V = 40000
+    rng = np.random.default_rng(44)
+    x = np.zeros((6, V), np.float32)
+    x[1, rng.permutation(V)[:300]] = 2.0
+    x[2] = rng.integers(0, 4, V) * 0.25
+    x[3] = -np.inf
+    x[3, 7::100] = 1.0  # 400 words in all
+    x[4, rng.permutation(V)[:1500]] = 4.0
+    x[5] = np.where(np.arange(V) < 600, 1.0, -np.inf)
+    u = np.array([0.0, 0.4, 0.71, 1.0 - 2.0 ** -24, np.nan, 0.9], np.float32)
+    tok, prob = lrs.sample(ctx, x, u, **opt)
+    check_rows(tok, prob, x, u, opt)
+
+
+@pytest.mark.parametrize("opt", [dict(top_k=300), dict(top_k=700, top_p=0.95), dict(top_p=0.5), dict(min_p=0.02),
+                                 dict(top_k=40, min_p=0.1)])
+def test_sample_random_number_edges_of_each_form(lrs, ctx, opt):
+    x = logits(np.random.default_rng(18), 1, 9001)[[0] * 8]
+    u = np.array([0.0, -0.0, -3.0, np.nan, 1.0 - 2.0 ** -24, 1.0, np.inf, 2.0 ** -149], np.float32)
+    tok, prob = lrs.sample(ctx, x, u, **opt)
+    check_rows(tok, prob, x, u, opt)
+
+
+@pytest.mark.parametrize("rows,vocab", [(700, 700), (300, 4500), (65, 33000)])
+def test_sample_many_rows_of_each_form(lrs, ctx, rows, vocab):
+    rng = np.random.default_rng(rows)
+    x, u = logits(rng, rows, vocab), rng.random(rows).astype(np.float32)
+    for opt in (dict(top_k=200, top_p=0.9), dict(top_k=1024), dict(top_p=0.8), dict(top_k=8, min_p=0.02)):
+        tok, prob = lrs.sample(ctx, x, u, **opt)
+        check_rows(tok, prob, x, u, opt)
+
+
 @pytest.mark.parametrize("opt", [dict(top_k=20), dict(top_p=0.8), dict()])
 def test_sample_random_number_edges(lrs, ctx, opt):
     x = logits(np.random.default_rng(8), 1, 3000)[[0] * 7]
@@ -578,4 +615,38 @@ def test_samplers_of_a_hybrid_model(lrs, orc, ctx):
     with pytest.raises(lrs.ModelError) as e:
         m.decode_tree([1, 2], [-1, 0], 1)
     assert e.value.code == -5
+    m.close()
+
+
+def test_logits_without_a_word(lrs, orc, ctx):
+    """a head whose logits are all NaN: an error, and the state says what is cached"""
+    def broken(w):
+        t, a = w["output"]
+        assert t == lrs.Q6_K
+        a = np.array(a, copy=True)
+        blocks = a.reshape(-1).view(np.uint8).reshape(-1, 210)
+        blocks[:, 208:] = np.frombuffer(np.float16(np.nan).tobytes(), np.uint8)
+        return dict(w, output=(t, a))
+
+    def fails(f, *a, **k):
+        with pytest.raises(lrs.ModelError) as e:
+            f(*a, **k)
+        assert e.value.code == -2 and "sampled" in str(e.value)
+
+    m = modelgen.gpu_model(lrs, ctx, modelgen.GQA5, broken(modelgen.host_model(orc, modelgen.GQA5, seed=11, mode=1)))
+    assert np.isnan(m.decode(3, 0)).all()
+    for opt in (dict(temperature=0.0), dict(top_k=10), dict(top_p=0.9)):
+        fails(m.decode_sample, 4, 1, 0.5, **opt)
+        assert len(m) == 2
+        fails(m.generate_sample, [4, 5, 6], [0.5] * 4, 1, **opt)
+        assert len(m) == 4
+        fails(m.verify_tree, [4, 5, 6], [-1, 0, 0], 1, u=[0.5] * 3, **opt)
+        assert len(m) == 1
+    m.close()
+    cfg = modelgen.HY_TINY
+    m = modelgen.gpu_hybrid_model(lrs, ctx, cfg, broken(modelgen.hybrid_host_model(orc, cfg, seed=3)))
+    fails(m.decode_sample, 4, 0, 0.5)
+    assert len(m) == 1
+    fails(m.generate_sample, [4, 5], [0.5] * 4, 1)
+    assert len(m) == 0
     m.close()
