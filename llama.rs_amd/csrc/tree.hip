@@ -187,6 +187,11 @@ __global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(
     // pieces are turned by the row (row >> VT & VM, times 4) so that those are in
     // different banks
     constexpr uint32_t VT = HD == 64 ? 1 : 0, VM = HD == 64 ? 1 : 3;
+    // tiles of a check for values that are not finite: at head_dim 256 one, whose
+    // registers are all taken (36 us with eight, 33 with one: 41 nodes behind 2047
+    // positions, 24 heads on 4 KV heads), else all (26 nodes of the 32B shape behind
+    // 3900 positions: no difference, but no spill)
+    constexpr int OC = HD == 256 ? 1 : OT;
     // K, then V of a group's chunk of even and of odd rounds; the groups' sums at the end
     __shared__ __attribute__((aligned(16))) _Float16 buf0[G][64 * HD], buf1[G][64 * HD];
     __shared__ float2 wml[G][T * 32];
@@ -339,21 +344,22 @@ __global__ __launch_bounds__(64 * T * G, tree_waves(HD, T, G)) void k_attn_tree(
             // a V that is not finite reaches the rows that see it alone: it is taken
             // out of the product (0 inf is NaN) and added where it is seen
             if (masked) {
-                u16x2_t top = {0, 0};
 #pragma unroll
-                for (int t = 0; t < OT; t++)
+                for (int t0 = 0; t0 < OT; t0 += OC) {
+                    u16x2_t top = {0, 0};
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
+                    for (int t = t0; t < t0 + OC; t++) {
                         const u16x8_t bits = __builtin_bit_cast(u16x8_t, va[t]) & (uint16_t)0x7FFF;
-                        top = __builtin_elementwise_max(top, u16x2_t{bits[j], bits[j + 1]});
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) top = __builtin_elementwise_max(top, u16x2_t{bits[j], bits[j + 1]});
                     }
-                if (__any(max(top[0], top[1]) >= 0x7C00)) {
+                    if (!__any(max(top[0], top[1]) >= 0x7C00)) continue;
                     f16x8_t one;
 #pragma unroll
                     for (int j = 0; j < 8; j++)
                         one[j] = mine >> (16 * s + 8 * (j >> 2) + (j & 3)) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
 #pragma unroll
-                    for (int t = 0; t < OT; t++) {
+                    for (int t = t0; t < t0 + OC; t++) {
 #pragma unroll 1
                         for (int kind = 0; kind < 3; kind++) {  // NaN, inf, -inf
                             f16x8_t is;
