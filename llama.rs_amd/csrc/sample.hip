@@ -998,6 +998,10 @@ uint32_t range_parts(uint32_t vocab, uint32_t rows, bool listed, uint32_t *part)
     return (vocab + *part - 1) / *part;
 }
 
+// The first form as far as its lists go: at top_k 128 a row of 32000 takes 18 us
+// against 23 with the second, 25 rows of 152064 26 against 36, 64 of 248320 46 against
+// 51; at top_k 40 10 against 23 for the row of 32000.  Listed as far as half a list: the
+// other half is for the rest of top-k's bin.
 struct Plan {
     bool first, listed;
     uint32_t e, parts, part, k;

@@ -542,7 +542,9 @@ __global__ __launch_bounds__(256) void k_tree_merge(AttnTree a, uint32_t hd, uin
 // of two tiles where there are two; a workgroup per CU, and two (the second
 // wavefront of a SIMD, whose products overlap the first's softmax) where a
 // wavefront then still has eight chunks: 64 nodes of the 32B shape behind 130000
-// positions 413 -> 369 us, 26 behind 3900 22 -> 26 us.
+// positions 413 -> 369 us, 26 behind 3900 22 -> 26 us.  One tile and twice the groups
+// where there are more tiles: 64 nodes 354 -> 578 us, 26 (five tiles) 22 -> 21, 8
+// behind 333 10.8 -> 11.6, 41 at head_dim 256 33 -> 34.
 struct TreeShape {
     uint32_t T, G, S;
 };
